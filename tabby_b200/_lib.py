@@ -1,7 +1,8 @@
-"""ctypes binding of libtabbysample.so (include/tabby_sample.h).
+"""ctypes binding of libtabbysample.so (include/tabby_sample.h) and libtabbydecode.so
+(include/tabby_decode.h).
 
-The library is the product: there is no Python or CPU fallback. If the shared object is
-missing or fails to load, ``lib()`` raises.
+The libraries are the product: there is no Python or CPU fallback. If a shared object is
+missing or fails to load, ``lib()`` and ``decode_lib()`` raise.
 """
 from __future__ import annotations
 
@@ -97,7 +98,65 @@ SIGNATURES = {
         [_P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _I32, _P], ctypes.c_int),
 }
 
+TABBY_BEAM_MAX = 64
+TABBY_BEAM_MAX_OUT = 128
+TABBY_TREE_MAX_NODES = 64
+TABBY_TREE_MAX_DIM = 128
+TABBY_F32, TABBY_BF16, TABBY_F16 = 0, 1, 2
+DECODE_LIB_PATH = os.path.join(_PKG, "lib", "libtabbydecode.so")
+
+
+class StateLayout(ctypes.Structure):
+    _fields_ = [
+        ("row_stride", _I64),
+        ("segment_stride", _I64),
+        ("entry_stride", _I64),
+        ("entry_bytes", _I64),
+        ("segments", _I32),
+        ("entries", _I32),
+    ]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        *[(n, _P) for n in ("q", "k", "v", "out")],
+        *[(f"{t}_{d}_stride", _I64) for t, ds in (("q", ("batch", "node", "head")),
+                                                  ("k", ("batch", "head", "entry")),
+                                                  ("v", ("batch", "head", "entry")),
+                                                  ("out", ("batch", "node", "head")))
+          for d in ds],
+        ("lengths", _P),
+        ("parents", _P),
+        ("parents_stride", _I64),
+        *[(n, _I32) for n in ("dtype", "batch", "nodes", "heads", "kv_heads", "dim", "entries")],
+        ("scale", _F32),
+        ("workspace", _P),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+# Every symbol include/tabby_decode.h declares, with its ctypes signature.
+DECODE_SIGNATURES = {
+    "tabby_decode_abi_version": ([], _I32),
+    "tabby_decode_last_error": ([], ctypes.c_char_p),
+    "tabby_beam_workspace_bytes": (
+        [_I32, _I32, _I32, _I32, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "tabby_beam_step_async": (
+        [_I32, _P, _I32, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32, _I32, _P, _P, _P, _P, _P,
+         _P, ctypes.c_size_t, _P], ctypes.c_int),
+    "tabby_states_reorder_async": (
+        [_I32, _P, _I32, ctypes.POINTER(StateLayout), _I32, _I32, _P, _P, _P], ctypes.c_int),
+    "tabby_tree_workspace_bytes": (
+        [_I32, _I32, _I32, _I32, _I32, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "tabby_tree_attention_async": (
+        [_I32, ctypes.POINTER(TreeAttentionArgs), _P], ctypes.c_int),
+    "tabby_tree_accept_async": (
+        [_I32, _P, _I64, _I64, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _I32,
+         ctypes.POINTER(StateLayout), _P], ctypes.c_int),
+}
+
 _lib = None
+_decode_lib = None
 
 
 class TabbyError(RuntimeError):
@@ -106,23 +165,39 @@ class TabbyError(RuntimeError):
         self.status = status
 
 
+def _load(path: str, signatures: dict) -> ctypes.CDLL:
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is missing; build it with `python -m tabby_b200.build`")
+    l = ctypes.CDLL(path)
+    for name, (args, res) in signatures.items():
+        fn = getattr(l, name)
+        fn.argtypes = args
+        fn.restype = res
+    return l
+
+
 def lib() -> ctypes.CDLL:
     """Load the shared library (raises if it is missing: no fallback exists)."""
     global _lib
     if _lib is None:
-        if not os.path.exists(LIB_PATH):
-            raise RuntimeError(
-                f"{LIB_PATH} is missing; build it with `python -m tabby_b200.build`"
-            )
-        l = ctypes.CDLL(LIB_PATH)
-        for name, (args, res) in SIGNATURES.items():
-            fn = getattr(l, name)
-            fn.argtypes = args
-            fn.restype = res
-        _lib = l
+        _lib = _load(LIB_PATH, SIGNATURES)
     return _lib
+
+
+def decode_lib() -> ctypes.CDLL:
+    """Load the decode operators' library (raises if it is missing: no fallback exists)."""
+    global _decode_lib
+    if _decode_lib is None:
+        _decode_lib = _load(DECODE_LIB_PATH, DECODE_SIGNATURES)
+    return _decode_lib
 
 
 def check(status: int) -> None:
     if status != TABBY_OK:
         raise TabbyError(status, lib().tabby_last_error().decode(errors="replace"))
+
+
+def check_decode(status: int) -> None:
+    if status != TABBY_OK:
+        raise TabbyError(status,
+                         decode_lib().tabby_decode_last_error().decode(errors="replace"))

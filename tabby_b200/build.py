@@ -1,9 +1,11 @@
-"""Build libtabbysample.so in-tree with nvcc for sm_100a.
+"""Build the shared libraries in-tree with nvcc for sm_100a.
 
-    python -m tabby_b200.build        # -> tabby_b200/lib/libtabbysample.so
+    python -m tabby_b200.build        # -> tabby_b200/lib/libtabby{sample,decode}.so
 
-The library is a plain C-ABI shared object (include/tabby_sample.h); it does not link
-against torch. CUDA's runtime is linked statically so the .so only needs the driver.
+libtabbysample.so (include/tabby_sample.h) is the sampler, libtabbydecode.so
+(include/tabby_decode.h) the decode operators for several hypotheses a sequence. Both are
+plain C-ABI shared objects that do not link against torch. CUDA's runtime is linked
+statically so they only need the driver.
 """
 from __future__ import annotations
 
@@ -11,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -19,7 +22,10 @@ LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libtabbysample.so")
 SOURCES = ["sampler_kernels.cu", "capi.cu", "noalloc.cu", "softmax_rows.cu", "lmhead.cu",
            "exchange.cu"]
-HEADERS = ["finalize.cuh", "js_math.cuh", "sampler_internal.h", "warp_sort.cuh"]
+DECODE_LIB = os.path.join(LIBDIR, "libtabbydecode.so")
+DECODE_SOURCES = ["decode_capi.cu", "beam.cu", "states.cu", "tree_attention.cu"]
+HEADERS = ["decode_internal.h", "finalize.cuh", "js_math.cuh", "sampler_internal.h",
+           "warp_sort.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -36,46 +42,53 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB):
+def _stale(lib: str, sources: list) -> bool:
+    if not os.path.exists(lib):
         return True
-    t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(ROOT, "include", "tabby_sample.h"))
+    t = os.path.getmtime(lib)
+    deps = [os.path.join(CSRC, f) for f in sources + HEADERS]
+    deps += [os.path.join(ROOT, "include", h) for h in ("tabby_sample.h", "tabby_decode.h")]
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
+
+
+def _run(cmd: list, what: str) -> str:
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what}:\n{r.stdout}\n{r.stderr}")
+    return r.stderr
+
+
+def _build_lib(lib_path: str, sources: list, verbose: bool, defines: tuple) -> None:
+    libdir = os.path.dirname(lib_path)
+    os.makedirs(libdir, exist_ok=True)
+    objs = [os.path.join(libdir, os.path.splitext(src)[0] + ".o") for src in sources]
+    cmds = [[nvcc(), *ARCH, *NVCC_FLAGS, *[f"-D{d}" for d in defines],
+             "-I", os.path.join(ROOT, "include"), "-I", CSRC,
+             "-c", os.path.join(CSRC, src), "-o", obj] for src, obj in zip(sources, objs)]
+    with ThreadPoolExecutor(max_workers=len(cmds)) as pool:  # a process a source
+        for err in pool.map(_run, cmds, [f"nvcc failed for {src}" for src in sources]):
+            if verbose:
+                sys.stderr.write(err)
+    tmp = lib_path + ".tmp"
+    _run([nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", tmp, *objs,
+          "-Xlinker", "--exclude-libs,ALL"], "link failed")
+    os.replace(tmp, lib_path)
+    for o in objs:
+        os.remove(o)
 
 
 def build(force: bool = False, verbose: bool = False, out: str | None = None,
           defines: tuple = ()) -> str:
-    """Compile SOURCES into `out` (default: the in-tree library). `defines` adds -D flags
-    (e.g. TABBY_CHECKS=1 for the self-checking debug build)."""
-    lib_path = out or LIB
-    if out is None and not force and not _stale():
-        return LIB
-    libdir = os.path.dirname(lib_path)
-    os.makedirs(libdir, exist_ok=True)
-    objs = []
-    for src in SOURCES:
-        obj = os.path.join(libdir, os.path.splitext(src)[0] + ".o")
-        cmd = [nvcc(), *ARCH, *NVCC_FLAGS, *[f"-D{d}" for d in defines],
-               "-I", os.path.join(ROOT, "include"), "-I", CSRC,
-               "-c", os.path.join(CSRC, src), "-o", obj]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed for {src}:\n{r.stdout}\n{r.stderr}")
-        if verbose:
-            sys.stderr.write(r.stderr)
-        objs.append(obj)
-    tmp = lib_path + ".tmp"
-    cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", tmp, *objs,
-           "-Xlinker", "--exclude-libs,ALL"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, lib_path)
-    for o in objs:
-        os.remove(o)
-    return lib_path
+    """Compile both libraries in-tree and return the sampler's path; with `out`, only
+    SOURCES into that path. `defines` adds -D flags (e.g. TABBY_CHECKS=1 for the
+    self-checking debug build)."""
+    if out is not None:
+        _build_lib(out, SOURCES, verbose, defines)
+        return out
+    for lib_path, sources in ((LIB, SOURCES), (DECODE_LIB, DECODE_SOURCES)):
+        if force or _stale(lib_path, sources):
+            _build_lib(lib_path, sources, verbose, defines)
+    return LIB
 
 
 if __name__ == "__main__":
