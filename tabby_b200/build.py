@@ -24,7 +24,7 @@ SOURCES = ["sampler_kernels.cu", "capi.cu", "noalloc.cu", "softmax_rows.cu", "lm
            "exchange.cu"]
 DECODE_LIB = os.path.join(LIBDIR, "libtabbydecode.so")
 DECODE_SOURCES = ["decode_capi.cu", "beam.cu", "states.cu", "tree_attention.cu"]
-HEADERS = ["decode_internal.h", "finalize.cuh", "js_math.cuh", "sampler_internal.h",
+HEADERS = ["decode_internal.h", "finalize.cuh", "js_math.cuh", "sampler_internal.h", "sm100.cuh",
            "warp_sort.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

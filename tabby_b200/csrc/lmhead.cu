@@ -34,7 +34,6 @@
 //                   table) and its merge run; both launches return at once otherwise.
 // Every mbarrier wait is bounded; a wait that runs out sets an error word and the rows
 // report TABBY_ETIMEOUT.
-#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
 #include <stdint.h>
@@ -42,9 +41,9 @@
 #include <string.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "sampler_internal.h"
+#include "sm100.cuh"
 #include "tabby_sample.h"
 #include "warp_sort.cuh"
 
@@ -62,7 +61,6 @@ constexpr int kWTileBytes = kLmN * kLmK * 2;  // 32 KB: a weight stage
 constexpr int kLmThreads = 320;    // TMA producer, MMA issuer, 8 epilogue warps
 constexpr int kEpiThreads = 256;   // two epilogue warps a TMEM lane quarter
 constexpr int kTmemCols = 2 * kLmN;
-constexpr unsigned long long kWaitNs = 500000000ull;  // a bounded wait gives up after 0.5 s
 // Candidate slots a row: its best 64 so far, sorted (slots 0-63), then up to 63 pending
 // composites above the 64th (slots 64-127), merged in by the warp once 32 are pending.
 constexpr int kLmBuf = 128;
@@ -108,125 +106,11 @@ struct LmArgs {
   uint32_t epoch;                // the call's tag: flags from earlier calls never match it
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void *p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void mb_init(uint64_t *b, uint32_t n) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(n) : "memory");
-}
-__device__ __forceinline__ void mb_arrive_expect(uint64_t *b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)),
-               "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void mb_arrive(uint64_t *b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
-}
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-__device__ __forceinline__ bool mb_try(uint64_t *b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_addr(b)), "r"(parity)
-      : "memory");
-  return ok != 0u;
-}
-// The clock is read only once a first attempt has failed (reading it costs tens of ns).
-__device__ __forceinline__ bool mb_wait(uint64_t *b, uint32_t parity) {
-  if (mb_try(b, parity)) return true;
-  const unsigned long long t0 = now_ns();
-  for (uint32_t i = 0;; i++) {
-    if ((i & 1023u) == 1023u && now_ns() - t0 > kWaitNs) return false;
-    if (mb_try(b, parity)) return true;
-  }
-}
-// 2-D TMA load of one box into this CTA's shared memory (coordinates: inner, outer).
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y,
-                                            uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
-      "{%3, %4}], [%2];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y)
-      : "memory");
-}
-// The same with an L2 cache policy: the weights are read once a call, so their lines go
-// first when L2 needs room and the small buffers and code the other kernels use stay.
-__device__ __forceinline__ uint64_t l2_evict_first() {
-  uint64_t pol;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
-  return pol;
-}
-__device__ __forceinline__ void tma_load_2d_hint(void *dst, const CUtensorMap *map, int x, int y,
-                                                 uint64_t *bar, uint64_t pol) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y), "l"(pol)
-      : "memory");
-}
-// Shared-memory matrix descriptor of a K-major tile written by TMA with 128-byte swizzle:
-// rows of 128 bytes, 8-row groups 1024 bytes apart (stride byte offset), descriptor
-// version 1 (sm_100), layout type 2 (SWIZZLE_128B). The tile base is 1024-byte aligned.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr >> 4) & 0x3FFFu);         // start address
-  d |= (uint64_t)1u << 16;                         // leading byte offset (unused here)
-  d |= (uint64_t)(1024u >> 4) << 32;               // stride byte offset
-  d |= (uint64_t)1u << 46;                         // version
-  d |= (uint64_t)2u << 61;                         // SWIZZLE_128B
-  return d;
-}
 // Instruction descriptor of kind::f16: bf16 A and B, fp32 accumulate, both K-major.
 // N (a multiple of 16, at most kLmN) is the tile's width.
 __device__ __forceinline__ uint32_t idesc_n(int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(kLmM >> 4) << 24);
-}
-
-__device__ __forceinline__ void mma_bf16(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
-                                         uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          smem_addr(bar))
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-      "%28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ex2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
 // Order-preserving key with -0 folded onto +0 (ties then go to the lower index), as the
@@ -458,7 +342,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
           const uint32_t ha = smem_addr(aring + sa * (int)a.a_bytes);
 #pragma unroll
           for (int kk = 0; kk < kLmK / 16; kk++)  // 16 bf16 = 32 bytes a step along K
-            mma_bf16(d, smem_desc(ha + 32 * kk), smem_desc(wa + 32 * kk), idesc,
+            mma_ss(d, smem_desc(ha + 32 * kk), smem_desc(wa + 32 * kk), idesc,
                    (kb | kk) != 0 ? 1u : 0u);
           mma_commit(&wempty[sw]);  // the stages are free once these MMAs have read them
           if (!a_res) mma_commit(&aempty[sa]);
@@ -772,25 +656,6 @@ __global__ void __launch_bounds__(kLmThreads, 1)
 }
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link to libcuda).
-using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                 const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_fn() {
-  static std::once_flag once;
-  static EncodeTiled fn = nullptr;
-  std::call_once(once, []() {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiled>(p);
-  });
-  return fn;
-}
-
 // K-major bf16 matrix [outer][inner] with boxes of 64 x box_rows (inner x outer), 128-byte
 // swizzle, zero fill out of bounds.
 bool make_map(CUtensorMap *m, const void *ptr, uint64_t inner, uint64_t outer, uint32_t box_rows) {
@@ -804,24 +669,6 @@ bool make_map(CUtensorMap *m, const void *ptr, uint64_t inner, uint64_t outer, u
              elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
          CUDA_SUCCESS;
-}
-
-// A launch with programmatic stream serialization: the kernel may start before the previous
-// one in the stream completes and orders itself with griddepcontrol.wait.
-template <typename... Args>
-cudaError_t launch_pdl(void (*kernel)(Args...), int grid, int block, size_t smem,
-                       cudaStream_t stream, const Args &...args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 int lfail(int status, const char *fmt, ...) {

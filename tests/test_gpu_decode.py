@@ -540,6 +540,17 @@ def test_tree_attention_ragged_batch(tb):
     check_attention(tb.tree_attention(q, k, v, lengths, parents), q, k, v, lengths, parents)
 
 
+@pytest.mark.parametrize("batch,length", [(296, 127), (592, 63), (592, 127), (300, 200),
+                                          (700, 90), (149, 500)])
+def test_tree_attention_many_sequences(tb, batch, length):
+    """More sequences than SMs: a worker goes through several of them, whole and in parts."""
+    q, k, v = attention_inputs(batch, 1, 2, 1, 64, length + 1, "bf16", batch)
+    lengths = torch.full((batch,), length, dtype=torch.int32, device="cuda")
+    lengths[::7] = length // 2
+    parents = torch.full((batch, 1), -1, dtype=torch.int32, device="cuda")
+    check_attention(tb.tree_attention(q, k, v, lengths, parents), q, k, v, lengths, parents)
+
+
 def test_tree_attention_unread_entries_may_hold_anything(tb):
     nodes = 12
     q, k, v = attention_inputs(4, nodes, 6, 2, 64, 160, "bf16", 5)
