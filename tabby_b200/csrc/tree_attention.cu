@@ -10,7 +10,7 @@
 // c = scale log2(e), m = c max S. The maximum is only moved when it rises by more than 8 in the exponent
 // (P then stays below 2^8), so O is rarely rescaled.
 //
-//   tree_kernel      one CTA a worker, two workers an SM, 192 threads. The work of a call --
+//   tree_kernel      one CTA a worker. The work of a call --
 //                    every (sequence, key/value head, row tile) has ceil((L + nodes) / 64) key
 //                    tiles -- is laid end to end and cut into equal ranges, one a worker, from
 //                    the lengths on the device: long and short sequences load the SMs evenly
@@ -21,7 +21,7 @@
 //                    warp 4      TMA producer: 4-D loads of K and V tiles (64 keys x 64 values
 //                                a box, 128-byte swizzle, zero fill past the cache) into two
 //                                rings.
-//                    warp 5      tcgen05.mma issuer: S double-buffered (the next tile's S is
+//                    last warps  tcgen05.mma issuers, one a row tile: S double-buffered (the next tile's S is
 //                                computed while this one's softmax runs), O in TMEM.
 //   tree_join_kernel joins the parts of items that were cut between workers.
 //
@@ -39,107 +39,128 @@ namespace {
 
 constexpr int kTileT = 64;        // keys a tile
 constexpr int kTileM = 128;       // query rows a tile (the MMA's M, TMEM's lanes)
-constexpr int kTreeThreads = 192;
 constexpr int kMaxWorkers = 320;  // bounds the workspace: two a SM
 constexpr float kLazy = 8.f;      // the maximum moves when it rises by more than 2^8
-constexpr int kTmemCols = 256;    // O: up to 128, S: 2 x 64
 
-// Shared memory of a worker for heads of up to DP values.
-template <int DP>
-struct TreeSmem {
+// A worker for heads of up to DP values that takes NS row tiles together: they share every K
+// and V tile. One row tile: two workers an SM; two: one.
+template <int DP, int NS>
+struct TreeCfg {
+  static constexpr int kThreads = 160 * NS + 32;
   static constexpr int kBlocks = DP / 64;             // blocks of 64 values: one swizzle row
-  static constexpr int kQ = kTileM * 128 * kBlocks;   // bytes of Q's tile
+  static constexpr int kQ = kTileM * 128 * kBlocks;   // bytes of a Q tile
   static constexpr int kKv = kTileT * 128 * kBlocks;  // bytes of a K or V tile
-  static constexpr int kStages = DP == 64 ? 4 : 2;    // tiles of each ring
-  static constexpr int kRings = 2 * kStages * kKv;
-  static constexpr size_t kBytes = 1024 + kQ + kRings + 1024;
+  static constexpr int kStages = NS == 1 ? (DP == 64 ? 5 : 2) : (DP == 64 ? 8 : 5);
+  static constexpr int kRings = 2 * kStages * kKv;    // K's and V's tiles
+  static constexpr size_t kSmem = 1024 + NS * kQ + kRings + 1024;
+  // TMEM columns: a row tile's O, then its two S tiles.
+  static constexpr uint32_t kO = 0, kS = NS * DP;
+  static constexpr uint32_t kTmem = NS == 1 ? 256 : 512;
+  static_assert(kS + NS * 2 * kTileT <= kTmem, "TMEM columns");
 };
 
 struct TreeArgs {
   tabby_tree_attention_args u;
   int32_t group;    // heads a key/value head
+  uint32_t by_group;  // ceil(2^32 / group): division by it as a product, group 2 to 256
   int32_t mrows;    // query rows of a key/value head
-  int32_t mtiles;   // row tiles of a key/value head
+  int32_t mtiles;   // row tiles of a key/value head, those that go together as one
   int32_t workers;  // CTAs the key tiles are cut over
-  int32_t prow;     // rows a part holds: min(mrows, 128)
+  int32_t prow;     // rows a part holds: min(mrows, 128 a row tile)
   float c;          // |scale| log2(e), 1 where scale is 0
   uint32_t q_xor;   // flips the signs of Q's values where scale is negative
   uint32_t q_and;   // 0 where scale is 0
-  float *part_o;    // [2 * workers][prow][dim]: unscaled sums
+  float *part_o;    // [2 * workers][dim / 4][prow][4]: unscaled sums
   float2 *part_ml;  // [2 * workers][prow]: m, sum
+  int2 *cuts;       // [items]: slot of the item's first part, its parts (0: not cut)
 };
 
+// y / group for a row y < 64 * group (and up to 255 more): with 2^32 / group rounded up the
+// product is above y / group by less than y / 2^32, below 1 / group while y * group < 2^32.
+__device__ __forceinline__ int div_group(const TreeArgs &a, int y) {
+  if (a.group == 1) return y;  // 2^32 has no place in by_group
+  return a.group <= 256 ? (int)__umulhi((uint32_t)y, a.by_group) : y / a.group;
+}
+
 // Key tiles of one (head, row tile) of a sequence; 0: nothing to attend to.
-__device__ __forceinline__ int64_t seq_tiles(const TreeArgs &a, int64_t b) {
-  const int64_t L = a.u.lengths[b];
+__device__ __forceinline__ int seq_tiles(const TreeArgs &a, int b) {
+  const int L = a.u.lengths[b];
   if (L < 0 || L >= a.u.entries) return 0;
-  const int64_t n = min(L + a.u.nodes, (int64_t)a.u.entries);
-  return (n + kTileT - 1) / kTileT;
+  const int n = a.u.entries - L > a.u.nodes ? L + a.u.nodes : a.u.entries;
+  return (n - 1) / kTileT + 1;
 }
-// All key tiles of the call (warp-uniform result; all lanes call).
-__device__ __forceinline__ int64_t all_tiles(const TreeArgs &a) {
-  int64_t n = 0;
-  for (int64_t b = threadIdx.x & 31; b < a.u.batch; b += 32) n += seq_tiles(a, b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n * a.u.kv_heads * a.mtiles;
-}
-// Where the tile `x` of the call lies: its sequence and the number of tiles before it (all
-// lanes call; x must be below all_tiles).
-__device__ __forceinline__ void find_tile(const TreeArgs &a, int64_t x, int64_t &b, int64_t &t0) {
+// Sums over the sequences, 32 at a time, a lane each; all lanes call. With x < 0: the key tiles
+// of the call. Else where tile x lies: its sequence, and the number of tiles before it.
+__device__ __forceinline__ int scan_tiles(const TreeArgs &a, int first32, int x, int &b) {
   const int lane = threadIdx.x & 31;
-  const int64_t per = (int64_t)a.u.kv_heads * a.mtiles;
-  t0 = 0;
-  for (int64_t b0 = 0; b0 < a.u.batch; b0 += 32) {
-    const int64_t n = b0 + lane < a.u.batch ? seq_tiles(a, b0 + lane) * per : 0;
-    int64_t end = n;  // inclusive prefix sum
+  const int per = a.u.kv_heads * a.mtiles;
+  int t0 = 0;
+  for (int b0 = 0; b0 < a.u.batch; b0 += 32) {
+    const int n = per * (b0 == 0 ? first32 : b0 + lane < a.u.batch ? seq_tiles(a, b0 + lane) : 0);
+    int end = n;  // inclusive prefix sum
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, end, o);
+      const int y = __shfl_up_sync(0xffffffffu, end, o);
       if (lane >= o) end += y;
     }
-    const unsigned in = __ballot_sync(0xffffffffu, n > 0 && t0 + end > x);
+    const unsigned in = __ballot_sync(0xffffffffu, x >= 0 && n > 0 && t0 + end > x);
     if (in) {
       const int f = __ffs(in) - 1;
       b = b0 + f;
-      t0 += __shfl_sync(0xffffffffu, end - n, f);
-      return;
+      return t0 + __shfl_sync(0xffffffffu, end - n, f);
     }
     t0 += __shfl_sync(0xffffffffu, end, 31);
   }
-  b = 0;  // not reached
+  return t0;
 }
-// How the tiles are cut: `n` workers, worker w from w * total / n on, none without a tile.
+// How the tiles are cut: `n` workers, worker w from floor(w * total / n) on, none without a
+// tile.
 struct Cut {
-  int64_t total, n;
-  __device__ __forceinline__ Cut(const TreeArgs &a)
-      : total(all_tiles(a)), n(min((int64_t)a.workers, total)) {}
-  __device__ __forceinline__ int64_t start(int64_t w) const { return w < n ? w * total / n : total; }
-  __device__ __forceinline__ int64_t worker(int64_t x) const { return ((x + 1) * n - 1) / total; }
+  int first32;  // the lane's share of the first 32 sequences' tiles
+  int total, n, q, rem;
+  __device__ __forceinline__ Cut(const TreeArgs &a) {
+    const int lane = threadIdx.x & 31;
+    int b;
+    first32 = lane < a.u.batch ? seq_tiles(a, lane) : 0;
+    total = scan_tiles(a, first32, -1, b);
+    n = min(a.workers, total);
+    q = n > 0 ? total / n : 0;
+    rem = total - q * n;
+  }
+  __device__ __forceinline__ int start(int w) const {
+    return w < n ? w * q + w * rem / n : total;
+  }
+  __device__ __forceinline__ int worker(int x) const {
+    return (int)((((int64_t)x + 1) * n - 1) / total);
+  }
 };
 
 // A worker's range, item after item: an item is (sequence, key/value head, row tile).
 struct Walk {
-  int64_t x, end;      // the next tile of the call, the range's end
-  int64_t b, nt;       // sequence, key tiles of an item
-  int32_t hk, mt;      // key/value head, row tile
-  int64_t t;           // the segment's first key tile
-  int64_t n;           // its key tiles
-  bool at_start;       // the segment begins the worker's range
+  int x, end;     // the next tile of the call, the range's end
+  int b, nt;      // sequence, key tiles of an item
+  int first;      // the item's first tile
+  int hk, mt;     // key/value head, row tile
+  int t;          // the segment's first key tile
+  int n;          // its key tiles
+  bool at_start;  // the segment begins the worker's range
 
   __device__ __forceinline__ void init(const TreeArgs &a, const Cut &cut, int w) {
     x = cut.start(w);
     end = cut.start(w + 1);
     at_start = true;
     if (x >= end) return;
-    int64_t t0;
-    find_tile(a, x, b, t0);
+    const int t0 = scan_tiles(a, cut.first32, x, b);
     nt = seq_tiles(a, b);
-    const int64_t item = (x - t0) / nt;
-    hk = (int32_t)(item / a.mtiles);
-    mt = (int32_t)(item % a.mtiles);
-    t = (x - t0) % nt;
+    const int item = (x - t0) / nt;
+    hk = item / a.mtiles;
+    mt = item - hk * a.mtiles;
+    t = x - t0 - item * nt;
+    first = x - t;
     n = min(nt - t, end - x);
+  }
+  __device__ __forceinline__ int64_t item(const TreeArgs &a) const {
+    return ((int64_t)b * a.u.kv_heads + hk) * a.mtiles + mt;
   }
   __device__ __forceinline__ bool more() const { return x < end; }
   __device__ __forceinline__ bool whole() const { return t == 0 && n == nt; }
@@ -156,6 +177,7 @@ struct Walk {
         while (nt == 0);
       }
     }
+    first = x;
     n = min(nt, end - x);
   }
 };
@@ -234,6 +256,29 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       : "memory");
 }
 
+// Packed and three-operand fp32 arithmetic.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  uint64_t r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "mov.b64 c, {%5, %6};\n\tfma.rn.f32x2 %0, a, b, c;\n\t}"
+      : "=l"(r)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
+  return make_float2(__uint_as_float((uint32_t)r), __uint_as_float((uint32_t)(r >> 32)));
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  uint64_t r;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "add.rn.f32x2 %0, a, b;\n\t}"
+      : "=l"(r)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return make_float2(__uint_as_float((uint32_t)r), __uint_as_float((uint32_t)(r >> 32)));
+}
+
 template <typename T> struct Half;
 template <> struct Half<__nv_bfloat16> {
   static constexpr uint32_t kType = 1;
@@ -255,51 +300,52 @@ template <> struct Half<__half> {
   }
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kTreeThreads, 2)
+template <typename T, int DP, int NS>
+__global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
     tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const __grid_constant__ TreeArgs a) {
-  typedef TreeSmem<DP> Smem;
-  constexpr int kStages = Smem::kStages;
-  constexpr uint32_t kO = 0, kS = DP;  // TMEM columns of O and of the two S tiles
+  typedef TreeCfg<DP, NS> Cfg;
+  constexpr int kStages = Cfg::kStages;
   extern __shared__ unsigned char smem_dyn[];
   unsigned char *base = reinterpret_cast<unsigned char *>(
       (reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
-  unsigned char *q_s = base, *k_s = base + Smem::kQ, *v_s = k_s + kStages * Smem::kKv;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(base + Smem::kQ + Smem::kRings);
+  unsigned char *q_s = base, *k_s = base + NS * Cfg::kQ, *v_s = k_s + kStages * Cfg::kKv;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(base + NS * Cfg::kQ + Cfg::kRings);
   uint64_t *kfull = bars, *kempty = kfull + kStages, *vfull = kempty + kStages,
-           *vempty = vfull + kStages, *sfull = vempty + kStages, *pready = sfull + 2,
-           *pvdone = pready + 2, *qfull = pvdone + 1, *drain = qfull + 1;
+           *vempty = vfull + kStages, *sfull = vempty + kStages, *pready = sfull + 2 * NS,
+           *pvdone = pready + 2 * NS, *qfull = pvdone + NS, *drain = qfull + NS;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   volatile uint32_t *err = tmem_slot + 1;
-  int32_t *parents = reinterpret_cast<int32_t *>(tmem_slot + 2);                 // [64]
-  uint32_t *used_bits = reinterpret_cast<uint32_t *>(parents + TABBY_TREE_MAX_NODES);  // [2]
+  int32_t *parents_s = reinterpret_cast<int32_t *>(tmem_slot + 2);  // [NS][64]
+  uint32_t *used_s = reinterpret_cast<uint32_t *>(parents_s + NS * TABBY_TREE_MAX_NODES);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     *err = 0;
     for (int i = 0; i < kStages; i++) {
       mb_init(&kfull[i], 1);
-      mb_init(&kempty[i], 1);
+      mb_init(&kempty[i], NS);
       mb_init(&vfull[i], 1);
-      mb_init(&vempty[i], 1);
+      mb_init(&vempty[i], NS);
     }
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < 2 * NS; i++) {
       mb_init(&sfull[i], 1);
       mb_init(&pready[i], 4);
     }
-    mb_init(pvdone, 1);
-    mb_init(qfull, 4);
-    mb_init(drain, 1);
+    for (int i = 0; i < NS; i++) {
+      mb_init(&pvdone[i], 1);
+      mb_init(&qfull[i], 4);
+    }
+    mb_init(drain, NS);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // The previous kernel of the stream is done from here on: nothing of it waits for the TMEM
   // columns that this CTA takes.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (warp == 5) {
+  if (warp == 4 * NS + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_addr(tmem_slot)),
-                 "n"(kTmemCols)
+                 "n"(Cfg::kTmem)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -313,25 +359,25 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
   Walk w;
   w.init(a, cut, blockIdx.x);
 
-  if (warp == 4) {
+  if (warp == 4 * NS) {
     // ---- TMA producer (one lane): K tiles one ahead of V tiles, as they are consumed ----
     if (lane == 0) {
       uint32_t ik = 0, iv = 0;  // tiles loaded so far
       bool ok = true;
       auto load = [&](uint64_t *full, uint64_t *empty, unsigned char *ring, uint32_t &i,
-                      const CUtensorMap *map, int64_t tile) {
+                      const CUtensorMap *map, int tile) {
         const uint32_t s = i % kStages;
         if (!mb_wait(&empty[s], ((i / kStages) & 1u) ^ 1u)) return false;
-        mb_arrive_expect(&full[s], (uint32_t)Smem::kKv);
-        for (int d = 0; d < Smem::kBlocks; d++)
-          tma_load_4d(ring + s * Smem::kKv + d * kTileT * 128, map, d * 64, (int)(tile * kTileT),
-                      w.hk, (int)w.b, &full[s]);
+        mb_arrive_expect(&full[s], (uint32_t)Cfg::kKv);
+        for (int d = 0; d < Cfg::kBlocks; d++)
+          tma_load_4d(ring + s * Cfg::kKv + d * kTileT * 128, map, d * 64, tile * kTileT, w.hk,
+                      w.b, &full[s]);
         i++;
         return true;
       };
       for (; w.more() && ok; w.next(a)) {
         ok = load(kfull, kempty, k_s, ik, &map_k, w.t);
-        for (int64_t t = 0; ok && t < w.n; t++) {
+        for (int t = 0; ok && t < w.n; t++) {
           if (*err) ok = false;
           if (ok && t + 1 < w.n) ok = load(kfull, kempty, k_s, ik, &map_k, w.t + t + 1);
           if (ok) ok = load(vfull, vempty, v_s, iv, &map_v, w.t + t);
@@ -344,55 +390,72 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
       for (uint32_t j = 0; j < min(iv, (uint32_t)kStages); j++)
         mb_wait(&vfull[(iv - 1 - j) % kStages], ((iv - 1 - j) / kStages) & 1u);
     }
-  } else if (warp == 5) {
-    // ---- MMA issuer: the warp goes along as one (so descriptors stay in uniform registers),
-    // an elected lane issues. K steps beyond the dim multiply zeros. ----
+  } else if (warp > 4 * NS) {
+    // ---- MMA issuers, a warp a row tile (while one waits, the other's products run). The warp
+    // goes along as one, so descriptors stay in uniform registers; an elected lane issues. K
+    // steps beyond the dim multiply zeros. ----
+    const int r = warp - 4 * NS - 1;
     constexpr uint32_t id_s = idesc_tree(Half<T>::kType, kTileT, 0u);
     constexpr uint32_t id_o = idesc_tree(Half<T>::kType, DP, 1u);
-    const uint64_t q_desc = smem_desc(smem_addr(q_s)), k_desc = smem_desc(smem_addr(k_s));
-    const uint64_t v_desc = smem_desc_v(smem_addr(v_s));  // in units of 16 bytes from here on
+    const uint64_t q_desc = smem_desc(smem_addr(q_s)) + r * (Cfg::kQ >> 4);
+    const uint64_t k_desc = smem_desc(smem_addr(k_s)), v_desc = smem_desc_v(smem_addr(v_s));
+    const uint32_t o_tm = tmem + Cfg::kO + r * DP, s_tm = tmem + Cfg::kS + 2 * r * kTileT;
+    uint64_t *sf = sfull + 2 * r, *pr = pready + 2 * r;
+    uint32_t ik = 0, iv = 0;           // K and V tiles of the worker
     uint32_t is = 0, io = 0, seg = 0;  // S tiles and O steps issued, segments begun
     bool ok = true;
-    auto issue_s = [&](int64_t t) {
-      const uint32_t s = is % kStages;
+    // The S tile of the segment's key tile t.
+    auto issue_s = [&](int t) {
+      const uint32_t s = ik % kStages;
       // S tile `is` takes the columns of P tile is - 2, which O step is - 2 has to have read.
       // (A segment's first tile finds every step done: Q's arrival stands behind them.)
-      if (t > 0 && is >= 2 && !wait_or(pvdone, (is - 2) & 1u, err)) return false;
-      if (!wait_or(&kfull[s], (is / kStages) & 1u, err)) return false;
+      if (t > 0 && is >= 2 && !wait_or(&pvdone[r], (is - 2) & 1u, err)) return false;
+      if (!wait_or(&kfull[s], (ik / kStages) & 1u, err)) return false;
       tc_fence_after();
-      const uint32_t d = tmem + kS + (is & 1u) * kTileT;
-      const uint64_t kd = k_desc + s * (Smem::kKv >> 4);
+      const uint64_t kd = k_desc + s * (Cfg::kKv >> 4);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; kk++)
-          mma_ss(d, q_desc + (kk >> 2) * (kTileM * 128 >> 4) + 2 * (kk & 3),
+          mma_ss(s_tm + (is & 1u) * kTileT, q_desc + (kk >> 2) * (kTileM * 128 >> 4) + 2 * (kk & 3),
                  kd + (kk >> 2) * (kTileT * 128 >> 4) + 2 * (kk & 3), id_s, kk != 0);
+        mma_commit(&sf[is & 1u]);
         mma_commit(&kempty[s]);
-        mma_commit(&sfull[is & 1u]);
       }
       __syncwarp();
+      ik++;
       is++;
       return true;
     };
-    for (; w.more() && ok; w.next(a), seg++) {
-      ok = wait_or(qfull, seg & 1u, err) && issue_s(0);
-      for (int64_t t = 0; ok && t < w.n; t++) {
-        if (ok && t + 1 < w.n) ok = issue_s(t + 1);
-        const uint32_t s = io % kStages;
-        ok = ok && wait_or(&vfull[s], (io / kStages) & 1u, err) &&
-             wait_or(&pready[io & 1u], (io >> 1) & 1u, err);
+    for (; w.more() && ok; w.next(a)) {
+      if ((w.mt * NS + r) * kTileM >= a.mrows) {  // no such row tile: only hands the tiles back
+        for (int t = 0; ok && t < w.n; t++, ik++, iv++) {
+          ok = wait_or(&kfull[ik % kStages], (ik / kStages) & 1u, err);
+          if (ok && lane == 0) mb_arrive(&kempty[ik % kStages]);
+          ok = ok && wait_or(&vfull[iv % kStages], (iv / kStages) & 1u, err);
+          if (ok && lane == 0) mb_arrive(&vempty[iv % kStages]);
+        }
+        continue;
+      }
+      ok = wait_or(&qfull[r], seg & 1u, err) && issue_s(0);
+      seg++;
+      for (int t = 0; ok && t < w.n; t++) {
+        if (t + 1 < w.n) ok = issue_s(t + 1);
+        const uint32_t s = iv % kStages;
+        ok = ok && wait_or(&vfull[s], (iv / kStages) & 1u, err) &&
+             wait_or(&pr[io & 1u], (io >> 1) & 1u, err);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t p = tmem + kS + (io & 1u) * kTileT;
-        const uint64_t vd = v_desc + s * (Smem::kKv >> 4);
+        const uint64_t vd = v_desc + s * (Cfg::kKv >> 4);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kTileT / 16; kk++)
-            mma_ts(tmem + kO, p + 8 * kk, vd + (2048 >> 4) * kk, id_o, t != 0 || kk != 0);
+            mma_ts(o_tm, s_tm + (io & 1u) * kTileT + 8 * kk, vd + (2048 >> 4) * kk, id_o,
+                   t != 0 || kk != 0);
+          mma_commit(&pvdone[r]);
           mma_commit(&vempty[s]);
-          mma_commit(pvdone);
         }
         __syncwarp();
+        iv++;
         io++;
       }
     }
@@ -401,105 +464,134 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     __syncwarp();
     wait_or(drain, 0, err);
   } else {
-    // ---- softmax, one row a thread ----
-    const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
+    // ---- softmax: four warps a row tile, one row a thread ----
+    const int rt = warp >> 2, r = tid & 127;  // row tile and row in it
+    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const uint32_t o_tm = lanes + Cfg::kO + rt * DP, s_tm = lanes + Cfg::kS + 2 * rt * kTileT;
+    int32_t *parents = parents_s + rt * TABBY_TREE_MAX_NODES;
+    uint32_t *used_bits = used_s + 2 * rt;
+    unsigned char *q_t = q_s + rt * Cfg::kQ;
     const float c = a.c;
     const int dim = a.u.dim;
-    uint32_t it = 0;  // tiles seen
+    uint32_t it = 0;   // tiles of the row tile
+    uint32_t itv = 0;  // V tiles of the worker
     bool ok = true;
-    for (; w.more(); w.next(a)) {
+    for (; w.more(); itv += (uint32_t)w.n, w.next(a)) {
       const int64_t L = a.u.lengths[w.b];
-      const int row = w.mt * kTileM + tid;       // of the key/value head's rows
-      const int node = row / a.group;
-      const int64_t head = w.hk * a.group + row % a.group;
+      const int row = (w.mt * NS + rt) * kTileM + r;  // of the key/value head's rows
+      if (row - r >= a.mrows) continue;               // no such row tile
+      int32_t parent = 0;
+      if (r < a.u.nodes) parent = a.u.parents[w.b * a.u.parents_stride + r];
+      const int node = div_group(a, row);
       const bool real = row < a.mrows;
-      // The tree: which slots the row sees, and which slots any row may see.
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (tid < a.u.nodes) parents[tid] = a.u.parents[w.b * a.u.parents_stride + tid];
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (warp < 2) {
-        const bool in = tid < a.u.nodes && L + tid < a.u.entries && tree_sees(parents, tid) != 0;
-        const uint32_t m = __ballot_sync(0xffffffffu, in);
-        if (lane == 0) used_bits[warp] = m;
-      }
-      unsigned long long sees = 0;
-      if (real && L + node < a.u.entries) sees = tree_sees(parents, node);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      const unsigned long long used =
-          (unsigned long long)used_bits[1] << 32 | (unsigned long long)used_bits[0];
+      constexpr int kPieces = DP / 8;  // of 16 bytes a row
+      const int row0 = row - r, piece = r % kPieces;
+      // Row `y` of the tile in the 16-bit tensor `p`: the thread's piece of it.
+      auto place = [&](const void *p, int y, int64_t batch, int64_t nodes, int64_t heads) {
+        const int n = div_group(a, y), g = y - n * a.group;
+        return const_cast<uint4 *>(reinterpret_cast<const uint4 *>(
+            static_cast<const T *>(p) + w.b * batch + n * nodes +
+            (int64_t)(w.hk * a.group + g) * heads + 8 * piece));
+      };
+      auto swizzled = [&](int y) {
+        return reinterpret_cast<uint4 *>(q_t + (piece >> 3) * (kTileM * 128) + y * 128 +
+                                         (((piece & 7) ^ (y & 7)) << 4));
+      };
       // Q's tile: 16-byte pieces at their swizzled places, zeros beyond the rows and the dim.
+      // All loads are on their way before the first is stored. (The tile's place is free: S's
+      // last tile is done, and the barrier stands behind the last result's way through it.)
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + rt) : "memory");
       if (ok) {
-        const T *q = static_cast<const T *>(a.u.q) + w.b * a.u.q_batch_stride +
-                     node * a.u.q_node_stride + head * a.u.q_head_stride;
+        uint4 x[kPieces];
 #pragma unroll
-        for (int p = 0; p < DP / 8; p++) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (real && 8 * p < dim) {
-            x = *reinterpret_cast<const uint4 *>(q + 8 * p);
-            x.x = (x.x ^ a.q_xor) & a.q_and;
-            x.y = (x.y ^ a.q_xor) & a.q_and;
-            x.z = (x.z ^ a.q_xor) & a.q_and;
-            x.w = (x.w ^ a.q_xor) & a.q_and;
-          }
-          *reinterpret_cast<uint4 *>(q_s + (p >> 3) * (kTileM * 128) + tid * 128 +
-                                     (((p & 7) ^ (tid & 7)) << 4)) = x;
+        for (int p = 0; p < kPieces; p++) {
+          const int y = row0 + r / kPieces + p * (128 / kPieces);
+          x[p] = make_uint4(0, 0, 0, 0);
+          if (y < a.mrows && 8 * piece < dim)
+            x[p] = *place(a.u.q, y, a.u.q_batch_stride, a.u.q_node_stride, a.u.q_head_stride);
+        }
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) {
+          x[p].x = (x[p].x ^ a.q_xor) & a.q_and;
+          x[p].y = (x[p].y ^ a.q_xor) & a.q_and;
+          x[p].z = (x[p].z ^ a.q_xor) & a.q_and;
+          x[p].w = (x[p].w ^ a.q_xor) & a.q_and;
+          const int y = r / kPieces + p * (128 / kPieces);
+          if (row0 + y >= a.mrows || 8 * piece >= dim) x[p] = make_uint4(0, 0, 0, 0);
+          *swizzled(y) = x[p];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mb_arrive(qfull);
+        if (lane == 0) mb_arrive(&qfull[rt]);
       }
+      // The tree: which slots the row sees, and which slots any row may see.
+      if (r < a.u.nodes) parents[r] = parent;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + rt) : "memory");
+      if ((warp & 3) < 2) {
+        const bool in = r < a.u.nodes && L + r < a.u.entries && tree_sees(parents, r) != 0;
+        const uint32_t m = __ballot_sync(0xffffffffu, in);
+        if (lane == 0) used_bits[warp & 3] = m;
+      }
+      unsigned long long sees = 0;
+      if (real && L + node < a.u.entries) sees = tree_sees(parents, node);
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + rt) : "memory");
+      const unsigned long long used =
+          (unsigned long long)used_bits[1] << 32 | (unsigned long long)used_bits[0];
       float m = -INFINITY, l = 0.f;  // m = c * maximum
-      for (int64_t t = 0; ok && t < w.n; t++, it++) {
+      for (int t = 0; ok && t < w.n; t++, it++) {
         const uint32_t sb = it & 1u;
-        if (!wait_or(&sfull[sb], (it >> 1) & 1u, err)) {
+        if (!wait_or(&sfull[2 * rt + sb], (it >> 1) & 1u, err)) {
           ok = false;
           break;
         }
         tc_fence_after();
         float s[64];
-        tmem_ld64(lanes + kS + sb * kTileT, s);
-        const int64_t t0 = (w.t + t) * kTileT;
+        tmem_ld64(s_tm + sb * kTileT, s);
+        const int64_t t0 = (int64_t)(w.t + t) * kTileT;
         if (t0 + kTileT > L) {
           // Keys behind the context: those the row sees. V's rows that no row sees may hold
-          // anything, and 0 times NaN is NaN: they become zeros.
-          auto place = [&](unsigned long long bits) -> unsigned long long {
+          // anything, and 0 times NaN is NaN: they become zeros before the O step.
+          auto at_tile = [&](unsigned long long bits) -> unsigned long long {
             if (L >= t0) {
               const int n = (int)(L - t0);  // below 64
-              return (1ull << n) - 1 | bits << n;
+              return ((1ull << n) - 1) | bits << n;
             }
             return t0 - L < 64 ? bits >> (t0 - L) : 0ull;
           };
-          const unsigned long long see = place(sees), any = place(used);
+          const unsigned long long see = at_tile(sees), any = at_tile(used);
 #pragma unroll
           for (int j = 0; j < 64; j++)
             if (!(see >> j & 1)) s[j] = -INFINITY;
-          const uint32_t vs = it % kStages;
-          if (!wait_or(&vfull[vs], (it / kStages) & 1u, err)) {
+          const uint32_t i = itv + (uint32_t)t, vs = i % kStages;
+          if (!wait_or(&vfull[vs], (i / kStages) & 1u, err)) {
             ok = false;
             break;
           }
-          if (!(any >> (tid & 63) & 1)) {
+          if (!(any >> (r & 63) & 1)) {
 #pragma unroll
-            for (int d = 0; d < Smem::kBlocks; d++)
+            for (int d = 0; d < Cfg::kBlocks; d++)
 #pragma unroll
               for (int p = 0; p < 4; p++)  // half a row a thread
-                *reinterpret_cast<uint4 *>(v_s + vs * Smem::kKv + d * kTileT * 128 +
-                                           (tid & 63) * 128 + (tid >> 6) * 64 + 16 * p) =
+                *reinterpret_cast<uint4 *>(v_s + vs * Cfg::kKv + d * kTileT * 128 +
+                                           (r & 63) * 128 + (r >> 6) * 64 + 16 * p) =
                     make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int j = 4; j < 64; j++) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        for (int j = 4; j < 60; j += 8)
+#pragma unroll
+          for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], s[j + 2 * i], s[j + 2 * i + 1]);
+        const float top = max3(max3(mx[0], mx[1], s[60]), max3(mx[2], mx[3], s[61]),
+                               fmaxf(s[62], s[63]));
         const bool rise = top * c - m > kLazy;
         if (t == 0) {
           m = top * c;
         } else if (__any_sync(0xffffffffu, rise)) {
           // O is free to change once its last step is done (the one before stood before this S
           // tile); this tile's is not yet issued.
-          if (!wait_or(pvdone, (it - 1) & 1u, err)) {
+          if (!wait_or(&pvdone[rt], (it - 1) & 1u, err)) {
             ok = false;
             break;
           }
@@ -508,80 +600,96 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
           m = rise ? top * c : m;
           l *= f;
 #pragma unroll 1
-          for (int d = 0; d < 16 * ((dim + 15) / 16); d += 32) {
+          for (int d = 0; d < dim; d += 32) {
             uint32_t o[32];
-            tmem_ld32(lanes + kO + d, o);
+            tmem_ld32(o_tm + d, o);
 #pragma unroll
             for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            tmem_st32(lanes + kO + d, o);
+            tmem_st32(o_tm + d, o);
           }
         }
         const float off = (m == -INFINITY ? 0.f : m) - Half<T>::kShift;
         uint32_t p[32];
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float2 sum[2] = {};
+        const float2 c2 = make_float2(c, c), off2 = make_float2(-off, -off);
 #pragma unroll
         for (int j = 0; j < 32; j++) {
-          const float x = ex2_fast(fmaf(s[2 * j], c, -off));
-          const float y = ex2_fast(fmaf(s[2 * j + 1], c, -off));
-          sum[(2 * j) & 3] += x;
-          sum[(2 * j + 1) & 3] += y;
-          p[j] = Half<T>::pack(x, y);
+          float2 x = fma2(make_float2(s[2 * j], s[2 * j + 1]), c2, off2);
+          x.x = ex2_fast(x.x);
+          x.y = ex2_fast(x.y);
+          sum[j & 1] = add2(sum[j & 1], x);
+          p[j] = Half<T>::pack(x.x, x.y);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st32(lanes + kS + sb * kTileT, p);
+        const float2 sums = add2(sum[0], sum[1]);
+        l += sums.x + sums.y;
+        tmem_st32(s_tm + sb * kTileT, p);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mb_arrive(&pready[sb]);
+        if (lane == 0) mb_arrive(&pready[2 * rt + sb]);
       }
       // The segment's result. S tile it - 1 stood behind O step it - 3: the last two are waited
       // for one after the other (a parity alone does not tell a step from the one two before).
-      if (ok && w.n > 1 && !wait_or(pvdone, (it - 2) & 1u, err)) ok = false;
-      if (ok && !wait_or(pvdone, (it - 1) & 1u, err)) ok = false;
+      if (ok && w.n > 1 && !wait_or(&pvdone[rt], (it - 2) & 1u, err)) ok = false;
+      if (ok && !wait_or(&pvdone[rt], (it - 1) & 1u, err)) ok = false;
       if (!ok) *err = 1;
       tc_fence_after();
       const bool whole = w.whole();
+      if (tid == 0 && w.t == 0)
+        a.cuts[w.item(a)] =
+            make_int2(2 * blockIdx.x + (w.at_start ? 0 : 1),
+                      whole ? 0 : (int)cut.worker(w.first + w.nt - 1) - (int)blockIdx.x + 1);
       const int64_t slot = 2 * (int64_t)blockIdx.x + (w.at_start ? 0 : 1);
-      const float inv = !ok ? NAN : 1.f / l;
-      T *out = static_cast<T *>(a.u.out) + w.b * a.u.out_batch_stride +
-               node * a.u.out_node_stride + head * a.u.out_head_stride;
-      float *part = a.part_o + (slot * a.prow + tid) * dim;
-      if (!whole && real) a.part_ml[slot * a.prow + tid] = make_float2(ok ? m : NAN, l);
+      const float inv = !ok ? NAN : sees == 0 ? 0.f : 1.f / l;
+      if (!whole && real) a.part_ml[slot * a.prow + rt * kTileM + r] = make_float2(ok ? m : NAN, l);
+      float4 *part = reinterpret_cast<float4 *>(a.part_o) + slot * (dim / 4) * a.prow +
+                     rt * kTileM + r;
 #pragma unroll
       for (int d = 0; d < DP; d += 32) {
         uint32_t o[32];
-        if (ok) {
-          tmem_ld32(lanes + kO + d, o);
-        } else {
+        tmem_ld32(o_tm + d, o);
+        if (whole) {  // rows through shared memory, so that they leave whole
 #pragma unroll
-          for (int j = 0; j < 32; j++) o[j] = 0x7fffffffu;
-        }
-        if (!real) continue;
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          if (d + j >= dim) continue;
-          if (whole) {
+          for (int j = 0; j < 32; j += 8) {
             uint32_t h[4];
 #pragma unroll
             for (int e = 0; e < 4; e++)
               h[e] = sees == 0 ? 0u
                                : Half<T>::pack(__uint_as_float(o[j + 2 * e]) * inv,
                                                __uint_as_float(o[j + 2 * e + 1]) * inv);
-            *reinterpret_cast<uint4 *>(out + d + j) = make_uint4(h[0], h[1], h[2], h[3]);
-          } else {
-            *reinterpret_cast<uint4 *>(part + d + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-            *reinterpret_cast<uint4 *>(part + d + j + 4) =
-                make_uint4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
+            const int pc = (d + j) / 8;
+            *reinterpret_cast<uint4 *>(q_t + (pc >> 3) * (kTileM * 128) + r * 128 +
+                                       (((pc & 7) ^ (r & 7)) << 4)) =
+                make_uint4(h[0], h[1], h[2], h[3]);
           }
+        } else if (real) {  // neighbouring rows lie side by side
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            if (d + j < dim)
+              part[(d + j) / 4 * a.prow] =
+                  make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]),
+                              __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
+        }
+      }
+      if (whole) {
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + rt) : "memory");
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) {
+          const int y = r / kPieces + p * (128 / kPieces);
+          if (row0 + y < a.mrows && 8 * piece < dim)
+            *place(a.u.out, row0 + y, a.u.out_batch_stride, a.u.out_node_stride,
+                   a.u.out_head_stride) = *swizzled(y);
         }
       }
       tc_fence_before();
     }
     // Sequences with nothing to attend to: zeros.
-    for (int64_t b = blockIdx.x; b < a.u.batch; b += gridDim.x) {
+    for (int b = blockIdx.x; b < a.u.batch; b += gridDim.x) {
       if (seq_tiles(a, b) != 0) continue;
+      for (int i = tid; i < a.u.kv_heads * a.mtiles; i += 128 * NS)
+        a.cuts[(int64_t)b * a.u.kv_heads * a.mtiles + i] = make_int2(0, 0);
       const int64_t per = (int64_t)a.u.heads * dim / 8;
-      for (int64_t i = tid; i < a.u.nodes * per; i += 128) {
-        T *out = static_cast<T *>(a.u.out) + b * a.u.out_batch_stride +
+      for (int64_t i = tid; i < a.u.nodes * per; i += 128 * NS) {
+        T *out = static_cast<T *>(a.u.out) + (int64_t)b * a.u.out_batch_stride +
                  i / per * a.u.out_node_stride + i % per / (dim / 8) * a.u.out_head_stride +
                  i % (dim / 8) * 8;
         *reinterpret_cast<uint4 *>(out) = make_uint4(0, 0, 0, 0);
@@ -590,76 +698,78 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 4 * NS + 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "n"(kTmemCols)
+                 "n"(Cfg::kTmem)
                  : "memory");
   }
 }
 
-// Joins the parts of the item that the start of worker blockIdx.x's range cuts first: weights
-// 2^(m_i - max m) for the parts' sums. A warp takes a row, its lanes 4 values each.
-template <typename T>
-__global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ TreeArgs a) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Cut cut(a);
-  const int64_t w = blockIdx.x, x = cut.start(w);
-  if (w == 0 || x >= cut.total) return;
-  int64_t b, t0;
-  find_tile(a, x, b, t0);
-  const int64_t nt = seq_tiles(a, b), item = (x - t0) / nt;
-  const int64_t first = t0 + item * nt;  // the item's first tile
-  const int64_t w0 = cut.worker(first), w1 = cut.worker(first + nt - 1);
-  if (w != w0 + 1) return;  // not the first cut of an item
-  const int hk = (int)(item / a.mtiles), mt = (int)(item % a.mtiles);
+// Joins the parts of the items that were cut between workers, with weights 2^(m_i - max m). A
+// part's sums lie as [group of 4 values][row]: a thread takes one place of them, neighbours
+// neighbouring ones, and goes through the parts; `share` threads share out the parts of a place
+// (few places, so that many parts are read at once).
+constexpr int kJoinThreads = 512;
+
+template <typename T, int NS>
+__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeArgs a,
+                                                                 int64_t items, int share) {
   __shared__ int32_t parents[TABBY_TREE_MAX_NODES];
-  if ((int)threadIdx.x < a.u.nodes)
-    parents[threadIdx.x] = a.u.parents[b * a.u.parents_stride + threadIdx.x];
-  __syncthreads();
-  const int64_t L = a.u.lengths[b];
-  const int rows = min(a.mrows - mt * kTileM, kTileM);
-  for (int r = blockIdx.y * 4 + warp; r < rows; r += gridDim.y * 4) {
-    const int row = mt * kTileM + r, node = row / a.group;
-    const int64_t head = (int64_t)hk * a.group + row % a.group;
-    const bool seen = L + node < a.u.entries && tree_sees(parents, node) != 0;
-    // Every part but the first begins its worker's range.
-    auto slot = [&](int64_t i) {
-      return 2 * i + (i == w0 && cut.start(w0) != first ? 1 : 0);
+  __shared__ float4 so[kJoinThreads];
+  __shared__ float2 sml[kJoinThreads];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, places = kJoinThreads / share;
+  const int first = tid / places;  // of the parts
+  const int at = (int)blockIdx.y * places + tid % places;
+  const int all = a.u.dim / 4 * a.prow;  // places of a part
+  const int g = at / a.prow, r = at - g * a.prow;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int mt = (int)(item % a.mtiles), hk = (int)(item / a.mtiles % a.u.kv_heads);
+    const int64_t b = item / a.mtiles / a.u.kv_heads;
+    const int2 cut = a.cuts[item];
+    const int64_t L = a.u.lengths[b];
+    int32_t parent = 0;
+    if (tid < a.u.nodes) parent = a.u.parents[b * a.u.parents_stride + tid];
+    const int n = cut.y;
+    if (n == 0) continue;
+    const int row = mt * NS * kTileM + r, node = div_group(a, row);
+    const bool real = at < all && row < a.mrows;
+    __syncthreads();
+    if (tid < a.u.nodes) parents[tid] = parent;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float m1, float l1, float4 y) {
+      const float m2 = fmaxf(m, m1);  // a NaN is passed over here, and kept by the sum
+      const float k = m == -INFINITY ? 0.f : ex2_fast(m - m2);
+      const float f = m1 == -INFINITY ? 0.f : ex2_fast(m1 - m2);
+      m = m2;
+      l = l * k + l1 * f;
+      o = make_float4(o.x * k + y.x * f, o.y * k + y.y * f, o.z * k + y.z * f, o.w * k + y.w * f);
     };
-    float m = -INFINITY;
-    bool bad = false;
-    for (int64_t i = w0 + lane; i <= w1; i += 32) {
-      const float y = a.part_ml[slot(i) * a.prow + r].x;
-      bad |= isnan(y);
-      m = fmaxf(m, y);
-    }
-    bad = __any_sync(0xffffffffu, bad);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t i = w0; i <= w1; i++) {
-      const float2 ml = a.part_ml[slot(i) * a.prow + r];
-      const float f = ml.x == -INFINITY ? 0.f : ex2_fast(ml.x - m);
-      l += f * ml.y;
-      if (4 * lane < a.u.dim) {
-        const float4 y = *reinterpret_cast<const float4 *>(
-            a.part_o + (slot(i) * a.prow + r) * a.u.dim + 4 * lane);
-        o[0] += f * y.x;
-        o[1] += f * y.y;
-        o[2] += f * y.z;
-        o[3] += f * y.w;
+    if (real) {
+#pragma unroll 4
+      for (int i = first; i < n; i += share) {
+        // The parts behind the first begin their workers' ranges: those have the even slots.
+        const int64_t slot = i == 0 ? cut.x : (cut.x & ~1) + 2 * i;
+        const float2 ml = a.part_ml[slot * a.prow + r];
+        add(ml.x, ml.y, reinterpret_cast<const float4 *>(a.part_o)[slot * all + at]);
       }
     }
-    if (4 * lane < a.u.dim) {
-      const float inv = bad ? NAN : 1.f / l;
+    so[tid] = o;
+    sml[tid] = make_float2(m, l);
+    __syncthreads();
+    if (real && first == 0) {
+      for (int i = 1; i < share; i++) add(sml[i * places + tid].x, sml[i * places + tid].y,
+                                          so[i * places + tid]);
+      const float inv = 1.f / l;
       uint2 h = make_uint2(0, 0);
-      if (seen)
-        h = make_uint2(Half<T>::pack(o[0] * inv, o[1] * inv), Half<T>::pack(o[2] * inv, o[3] * inv));
+      if (L + node < a.u.entries && tree_sees(parents, node) != 0)
+        h = make_uint2(Half<T>::pack(o.x * inv, o.y * inv), Half<T>::pack(o.z * inv, o.w * inv));
+      const int64_t head = (int64_t)hk * a.group + row - node * a.group;
       *reinterpret_cast<uint2 *>(static_cast<T *>(a.u.out) + b * a.u.out_batch_stride +
-                                 node * a.u.out_node_stride + head * a.u.out_head_stride +
-                                 4 * lane) = h;
+                                 node * a.u.out_node_stride + head * a.u.out_head_stride + 4 * g) =
+          h;
     }
   }
 }
@@ -719,34 +829,46 @@ DeviceInfo device_info() {
   if ((d.err = cudaGetDevice(&dev)) != cudaSuccess) return d;
   std::lock_guard<std::mutex> lock(mu);
   if (dev < kDevices && info[dev].err == cudaSuccess) return info[dev];
-  auto set = [](const void *f, size_t bytes) {
-    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  d.err = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
+  auto set = [&](auto *f, size_t bytes) {
+    if (d.err == cudaSuccess)
+      d.err = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   };
-  if ((d.err = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev)) ==
-          cudaSuccess &&
-      (d.err = set((const void *)tree_kernel<__nv_bfloat16, 64>, TreeSmem<64>::kBytes)) ==
-          cudaSuccess &&
-      (d.err = set((const void *)tree_kernel<__nv_bfloat16, 128>, TreeSmem<128>::kBytes)) ==
-          cudaSuccess &&
-      (d.err = set((const void *)tree_kernel<__half, 64>, TreeSmem<64>::kBytes)) == cudaSuccess &&
-      (d.err = set((const void *)tree_kernel<__half, 128>, TreeSmem<128>::kBytes)) ==
-          cudaSuccess &&
-      dev < kDevices)
-    info[dev] = d;
+  set(tree_kernel<__nv_bfloat16, 64, 1>, TreeCfg<64, 1>::kSmem);
+  set(tree_kernel<__nv_bfloat16, 64, 2>, TreeCfg<64, 2>::kSmem);
+  set(tree_kernel<__nv_bfloat16, 128, 1>, TreeCfg<128, 1>::kSmem);
+  set(tree_kernel<__nv_bfloat16, 128, 2>, TreeCfg<128, 2>::kSmem);
+  set(tree_kernel<__half, 64, 1>, TreeCfg<64, 1>::kSmem);
+  set(tree_kernel<__half, 64, 2>, TreeCfg<64, 2>::kSmem);
+  set(tree_kernel<__half, 128, 1>, TreeCfg<128, 1>::kSmem);
+  set(tree_kernel<__half, 128, 2>, TreeCfg<128, 2>::kSmem);
+  if (d.err == cudaSuccess && dev < kDevices) info[dev] = d;
   return d;
 }
 
-template <typename T>
+template <typename T, int DP, int NS>
 cudaError_t launch_tree(const TreeArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
                         cudaStream_t s) {
-  cudaError_t err =
-      a.u.dim <= 64
-          ? launch_pdl(tree_kernel<T, 64>, a.workers, kTreeThreads, TreeSmem<64>::kBytes, s, mk,
-                       mv, a)
-          : launch_pdl(tree_kernel<T, 128>, a.workers, kTreeThreads, TreeSmem<128>::kBytes, s, mk,
-                       mv, a);
+  typedef TreeCfg<DP, NS> Cfg;
+  const cudaError_t err = launch_pdl(tree_kernel<T, DP, NS>, a.workers, Cfg::kThreads, Cfg::kSmem,
+                                     s, mk, mv, a);
   if (err != cudaSuccess) return err;
-  return launch_pdl(tree_join_kernel<T>, dim3(a.workers, (a.prow + 15) / 16), 128, 0, s, a);
+  const int64_t items = (int64_t)a.u.batch * a.u.kv_heads * a.mtiles;
+  const int all = a.u.dim / 4 * a.prow;
+  const int share = all <= 1024 ? 8 : 1;  // a few rows: the parts are shared out
+  const int places = kJoinThreads / share;
+  return launch_pdl(tree_join_kernel<T, NS>,
+                    dim3((unsigned)std::min<int64_t>(items, a.workers),
+                         (unsigned)((all + places - 1) / places)),
+                    kJoinThreads, 0, s, a, items, share);
+}
+
+template <typename T>
+cudaError_t launch_tree_of(const TreeArgs &a, int ns, const CUtensorMap &mk, const CUtensorMap &mv,
+                           cudaStream_t s) {
+  if (a.u.dim <= 64)
+    return ns == 1 ? launch_tree<T, 64, 1>(a, mk, mv, s) : launch_tree<T, 64, 2>(a, mk, mv, s);
+  return ns == 1 ? launch_tree<T, 128, 1>(a, mk, mv, s) : launch_tree<T, 128, 2>(a, mk, mv, s);
 }
 
 }  // namespace
@@ -760,8 +882,11 @@ int tabby_tree_workspace_bytes(int32_t batch, int32_t nodes, int32_t heads, int3
   const int st = check_tree(batch, nodes, heads, kv_heads, dim);
   if (st) return st;
   if (!bytes) return decode_fail(TABBY_EINVAL, "tree_attention: bytes is NULL");
-  const size_t rows = (size_t)std::min<int64_t>((int64_t)nodes * (heads / kv_heads), kTileM);
-  *bytes = 2 * (size_t)kMaxWorkers * rows * (sizeof(float2) + (size_t)dim * sizeof(float));
+  const size_t rows = (size_t)std::min<int64_t>((int64_t)nodes * (heads / kv_heads), 2 * kTileM);
+  const size_t items = (size_t)batch * kv_heads *
+                       (((size_t)nodes * (heads / kv_heads) + kTileM - 1) / kTileM);
+  *bytes = 2 * (size_t)kMaxWorkers * rows * (sizeof(float2) + (size_t)dim * sizeof(float)) +
+           items * sizeof(int2);
   return TABBY_OK;
 }
 
@@ -810,23 +935,29 @@ int tabby_tree_attention_async(int32_t device, const tabby_tree_attention_args *
   t.u = a;
   t.group = a.heads / a.kv_heads;
   t.mrows = a.nodes * t.group;
-  t.mtiles = (t.mrows + kTileM - 1) / kTileM;
-  t.prow = std::min(t.mrows, kTileM);
+  const int ns = t.mrows > kTileM ? 2 : 1;  // row tiles that go together
+  t.mtiles = (t.mrows + ns * kTileM - 1) / (ns * kTileM);
+  t.prow = std::min(t.mrows, ns * kTileM);
+  t.by_group = (uint32_t)((((uint64_t)1 << 32) + t.group - 1) / t.group);
   const double most = (double)a.batch * a.kv_heads * t.mtiles *
                       (((double)a.entries + kTileT - 1) / kTileT);
-  t.workers = (int32_t)std::min<double>(std::min(2 * info.sms, kMaxWorkers), std::max(1.0, most));
+  if (most > 2147483647.0)
+    return decode_fail(TABBY_EINVAL, "tree_attention: batch * kv_heads * entries is too large");
+  t.workers = (int32_t)std::min<double>(std::min((ns == 1 ? 2 : 1) * info.sms, kMaxWorkers),
+                                         std::max(1.0, most));
   t.c = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
   t.q_xor = a.scale < 0.f ? 0x80008000u : 0u;
   t.q_and = a.scale == 0.f ? 0u : 0xffffffffu;
   t.part_o = static_cast<float *>(a.workspace);
   t.part_ml = reinterpret_cast<float2 *>(t.part_o + 2 * (size_t)kMaxWorkers * t.prow * a.dim);
+  t.cuts = reinterpret_cast<int2 *>(t.part_ml + 2 * (size_t)kMaxWorkers * t.prow);
   CUtensorMap mk, mv;
   if (!make_cache_map(&mk, a.k, a, a.k_batch_stride, a.k_head_stride, a.k_entry_stride) ||
       !make_cache_map(&mv, a.v, a, a.v_batch_stride, a.v_head_stride, a.v_entry_stride))
     return decode_fail(TABBY_EINVAL, "tree_attention: the caches' layout has no tensor map");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = a.dtype == TABBY_BF16 ? launch_tree<__nv_bfloat16>(t, mk, mv, s)
-                                                : launch_tree<__half>(t, mk, mv, s);
+  const cudaError_t err = a.dtype == TABBY_BF16 ? launch_tree_of<__nv_bfloat16>(t, ns, mk, mv, s)
+                                                : launch_tree_of<__half>(t, ns, mk, mv, s);
   if (err != cudaSuccess) return decode_cuda_fail(err, "tree_attention launch");
   return TABBY_OK;
 }
