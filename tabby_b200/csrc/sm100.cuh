@@ -56,6 +56,7 @@ __device__ __forceinline__ bool mb_wait(uint64_t *b, uint32_t parity) {
 // True on one lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
+  __syncwarp();
   asm volatile(
       "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(p));
@@ -112,8 +113,10 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
       : "memory");
 }
 // 32 columns of the warp's lanes; the values are there when it returns (the wait is part of the
-// statement, so no use of them can be moved before it).
+// statement, so no use of them can be moved before it). The access is aligned: the warp has to
+// be converged, whatever branch stood before.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  __syncwarp();
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
       "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "

@@ -221,8 +221,10 @@ __host__ __device__ constexpr uint32_t idesc_tree(uint32_t type, int n, uint32_t
   return (1u << 4) | (type << 7) | (type << 10) | (b_n_major << 16) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(kTileM >> 4) << 24);
 }
-// 64 columns of the warp's lanes; the values are there when it returns.
+// 64 columns of the warp's lanes; the values are there when it returns. (TMEM accesses are
+// aligned: the warp has to be converged, so each stands behind a __syncwarp.)
 __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
+  __syncwarp();
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
       "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
@@ -244,6 +246,7 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  __syncwarp();
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
       "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
@@ -313,7 +316,7 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
   uint64_t *bars = reinterpret_cast<uint64_t *>(base + NS * Cfg::kQ + Cfg::kRings);
   uint64_t *kfull = bars, *kempty = kfull + kStages, *vfull = kempty + kStages,
            *vempty = vfull + kStages, *sfull = vempty + kStages, *pready = sfull + 2 * NS,
-           *pvdone = pready + 2 * NS, *qfull = pvdone + NS, *drain = qfull + NS;
+           *pvdone = pready + 2 * NS, *qfull = pvdone + 2 * NS, *drain = qfull + NS;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   volatile uint32_t *err = tmem_slot + 1;
   int32_t *parents_s = reinterpret_cast<int32_t *>(tmem_slot + 2);  // [NS][64]
@@ -331,11 +334,9 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
     for (int i = 0; i < 2 * NS; i++) {
       mb_init(&sfull[i], 1);
       mb_init(&pready[i], 4);
-    }
-    for (int i = 0; i < NS; i++) {
       mb_init(&pvdone[i], 1);
-      mb_init(&qfull[i], 4);
     }
+    for (int i = 0; i < NS; i++) mb_init(&qfull[i], 4);
     mb_init(drain, NS);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -400,7 +401,9 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
     const uint64_t q_desc = smem_desc(smem_addr(q_s)) + r * (Cfg::kQ >> 4);
     const uint64_t k_desc = smem_desc(smem_addr(k_s)), v_desc = smem_desc_v(smem_addr(v_s));
     const uint32_t o_tm = tmem + Cfg::kO + r * DP, s_tm = tmem + Cfg::kS + 2 * r * kTileT;
-    uint64_t *sf = sfull + 2 * r, *pr = pready + 2 * r;
+    // One barrier for the even and one for the odd tiles of each kind: who waits is never two
+    // phases of a barrier behind, so a phase's parity tells it.
+    uint64_t *sf = sfull + 2 * r, *pr = pready + 2 * r, *pd = pvdone + 2 * r;
     uint32_t ik = 0, iv = 0;           // K and V tiles of the worker
     uint32_t is = 0, io = 0, seg = 0;  // S tiles and O steps issued, segments begun
     bool ok = true;
@@ -409,7 +412,7 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
       const uint32_t s = ik % kStages;
       // S tile `is` takes the columns of P tile is - 2, which O step is - 2 has to have read.
       // (A segment's first tile finds every step done: Q's arrival stands behind them.)
-      if (t > 0 && is >= 2 && !wait_or(&pvdone[r], (is - 2) & 1u, err)) return false;
+      if (t > 0 && is >= 2 && !wait_or(&pd[is & 1u], ((is - 2) >> 1) & 1u, err)) return false;
       if (!wait_or(&kfull[s], (ik / kStages) & 1u, err)) return false;
       tc_fence_after();
       const uint64_t kd = k_desc + s * (Cfg::kKv >> 4);
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
           for (int kk = 0; kk < kTileT / 16; kk++)
             mma_ts(o_tm, s_tm + (io & 1u) * kTileT + 8 * kk, vd + (2048 >> 4) * kk, id_o,
                    t != 0 || kk != 0);
-          mma_commit(&pvdone[r]);
+          mma_commit(&pd[io & 1u]);
           mma_commit(&vempty[s]);
         }
         __syncwarp();
@@ -468,6 +471,7 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
     const int rt = warp >> 2, r = tid & 127;  // row tile and row in it
     const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     const uint32_t o_tm = lanes + Cfg::kO + rt * DP, s_tm = lanes + Cfg::kS + 2 * rt * kTileT;
+    uint64_t *pd = pvdone + 2 * rt;
     int32_t *parents = parents_s + rt * TABBY_TREE_MAX_NODES;
     uint32_t *used_bits = used_s + 2 * rt;
     unsigned char *q_t = q_s + rt * Cfg::kQ;
@@ -483,7 +487,7 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
       int32_t parent = 0;
       if (r < a.u.nodes) parent = a.u.parents[w.b * a.u.parents_stride + r];
       const int node = div_group(a, row);
-      const bool real = row < a.mrows;
+      const bool real = row < a.mrows, idle = row - lane >= a.mrows;  // idle: the whole warp
       constexpr int kPieces = DP / 8;  // of 16 bytes a row
       const int row0 = row - r, piece = r % kPieces;
       // Row `y` of the tile in the 16-bit tensor `p`: the thread's piece of it.
@@ -546,28 +550,26 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
         }
         tc_fence_after();
         float s[64];
-        tmem_ld64(s_tm + sb * kTileT, s);
+        if (!idle) tmem_ld64(s_tm + sb * kTileT, s);
         const int64_t t0 = (int64_t)(w.t + t) * kTileT;
-        if (t0 + kTileT > L) {
-          // Keys behind the context: those the row sees. V's rows that no row sees may hold
-          // anything, and 0 times NaN is NaN: they become zeros before the O step.
-          auto at_tile = [&](unsigned long long bits) -> unsigned long long {
-            if (L >= t0) {
-              const int n = (int)(L - t0);  // below 64
-              return ((1ull << n) - 1) | bits << n;
-            }
-            return t0 - L < 64 ? bits >> (t0 - L) : 0ull;
-          };
-          const unsigned long long see = at_tile(sees), any = at_tile(used);
-#pragma unroll
-          for (int j = 0; j < 64; j++)
-            if (!(see >> j & 1)) s[j] = -INFINITY;
+        const bool tail = t0 + kTileT > L;  // the tile holds keys behind the context
+        // A slot mask as one over the tile's keys, those of the context set.
+        auto at_tile = [&](unsigned long long bits) -> unsigned long long {
+          if (L >= t0) {
+            const int n = (int)(L - t0);  // below 64
+            return ((1ull << n) - 1) | bits << n;
+          }
+          return t0 - L < 64 ? bits >> (t0 - L) : 0ull;
+        };
+        if (tail) {
+          // V's rows that no query row sees may hold anything, and 0 times NaN is NaN: they
+          // become zeros before the O step.
           const uint32_t i = itv + (uint32_t)t, vs = i % kStages;
           if (!wait_or(&vfull[vs], (i / kStages) & 1u, err)) {
             ok = false;
             break;
           }
-          if (!(any >> (r & 63) & 1)) {
+          if (!(at_tile(used) >> (r & 63) & 1)) {
 #pragma unroll
             for (int d = 0; d < Cfg::kBlocks; d++)
 #pragma unroll
@@ -577,6 +579,17 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
                     make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        if (idle) {  // P's rows of this warp reach only its own rows of O, which nobody reads
+          __syncwarp();
+          if (lane == 0) mb_arrive(&pready[2 * rt + sb]);
+          continue;
+        }
+        if (tail) {
+          const unsigned long long see = at_tile(sees);
+#pragma unroll
+          for (int j = 0; j < 64; j++)
+            if (!(see >> j & 1)) s[j] = -INFINITY;
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -589,9 +602,8 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
         if (t == 0) {
           m = top * c;
         } else if (__any_sync(0xffffffffu, rise)) {
-          // O is free to change once its last step is done (the one before stood before this S
-          // tile); this tile's is not yet issued.
-          if (!wait_or(&pvdone[rt], (it - 1) & 1u, err)) {
+          // O is free to change once its last step is done; this tile's is not yet issued.
+          if (!wait_or(&pd[(it - 1) & 1u], ((it - 1) >> 1) & 1u, err)) {
             ok = false;
             break;
           }
@@ -627,10 +639,8 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
         __syncwarp();
         if (lane == 0) mb_arrive(&pready[2 * rt + sb]);
       }
-      // The segment's result. S tile it - 1 stood behind O step it - 3: the last two are waited
-      // for one after the other (a parity alone does not tell a step from the one two before).
-      if (ok && w.n > 1 && !wait_or(&pvdone[rt], (it - 2) & 1u, err)) ok = false;
-      if (ok && !wait_or(&pvdone[rt], (it - 1) & 1u, err)) ok = false;
+      // The segment's result, behind its last O step.
+      if (ok && !wait_or(&pd[(it - 1) & 1u], ((it - 1) >> 1) & 1u, err)) ok = false;
       if (!ok) *err = 1;
       tc_fence_after();
       const bool whole = w.whole();
@@ -810,7 +820,7 @@ bool make_cache_map(CUtensorMap *m, const void *ptr, const tabby_tree_attention_
              a.dtype == TABBY_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
              4, const_cast<void *>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

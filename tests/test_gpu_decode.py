@@ -505,7 +505,7 @@ def attention_inputs(batch, nodes, heads, kv_heads, dim, entries, dtype, seed, t
 @pytest.mark.parametrize("nodes,heads,kv_heads,dim", [
     (1, 1, 1, 64), (1, 14, 2, 64), (2, 15, 5, 64), (5, 8, 8, 128), (26, 14, 2, 64),
     (64, 8, 2, 128), (33, 4, 1, 80), (17, 6, 3, 8), (64, 12, 1, 64), (7, 9, 3, 104),
-    (3, 64, 1, 16), (64, 64, 1, 128), (64, 7, 7, 72),
+    (3, 64, 1, 16), (64, 64, 1, 128), (64, 7, 7, 72), (2, 300, 1, 16), (3, 257, 1, 64),
 ])
 def test_tree_attention_matches_the_definition(tb, nodes, heads, kv_heads, dim, dtype):
     lens = [0, 1, 63, 64, 65, 200]
@@ -667,6 +667,22 @@ def test_tree_attention_streams_and_graphs(tb):
     torch.cuda.synchronize()
     assert torch.equal(res[0], res[1])
     check_attention(res[0], q, k, v, lengths, parents)
+
+
+@pytest.mark.parametrize("batch,nodes,heads,kv_heads,dim,length", [
+    (12, 9, 14, 2, 64, 3000), (6, 26, 32, 8, 128, 1500), (8, 1, 32, 8, 128, 2500),
+    (2, 64, 16, 4, 128, 2000),
+])
+def test_tree_attention_repeats_bit_for_bit(tb, batch, nodes, heads, kv_heads, dim, length):
+    """Many runs on ranges of several tiles: what the kernel's warps wait for must not depend
+    on how fast each of them is."""
+    q, k, v = attention_inputs(batch, nodes, heads, kv_heads, dim, length + nodes, "bf16", 40)
+    lengths = torch.randint(0, length, (batch,), device="cuda", generator=gen(2)).int()
+    parents = random_trees(batch, nodes, 6)
+    first = tb.tree_attention(q, k, v, lengths, parents)
+    check_attention(first, q, k, v, lengths, parents)
+    for _ in range(150):
+        assert torch.equal(first, tb.tree_attention(q, k, v, lengths, parents))
 
 
 def test_tree_attention_refusals(tb):
