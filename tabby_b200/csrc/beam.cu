@@ -3,17 +3,43 @@
 //
 //   lse(i) = max + log(sum exp(x - max)),  key(i, v) = score(i) + (x - lse(i)) in 64 bits
 //
-// beam_row_kernel: one CTA a row; maximum, sum, then the row's n best logits one after the
-// other, each a pass over the row (the best one behind the last in the order value falling,
-// index rising). beam_pick_kernel: one CTA a prompt merges its rows' lists the same way.
+//   beam_scan_kernel  reads every logit once. A CTA of 256 threads takes a chunk of a row (8192
+//                     logits, or 4096 where there are few rows) into registers, all loads at
+//                     once; the chunk's maximum, its sum of exponentials and the logits that
+//                     can be among its n_out best are found from there. A bound on the n_out-th
+//                     best: of the 8 warps' thread maxima the ceil(n_out / 8) best each are at
+//                     least n_out logits, so all that matters is no smaller than the least of
+//                     them. Where more logits than a list holds pass it (ties, or warps without
+//                     logits) the exact n_out-th best is found by bisection over the values.
+//   beam_pick_kernel  a CTA a prompt: the beams' log-sum-exps from the chunks' statistics, the
+//                     keys of the listed logits, the n_out best of them.
+//
+// The sums of a chunk are in fp32, so a lse is off by up to gap / 2 (gap_of below), and keys of
+// different beams that are closer than the gap might be out of order. Such pairs are rare; where
+// the sorted result has one, the lse of the beams in it is computed again in 64 bits from all
+// their logits (the rows are read once more) and the listed keys are sorted again.
 #include <math.h>
 
+#include <algorithm>
+
 #include "decode_internal.h"
+#include "sm100.cuh"
 
 namespace tabby {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kScanThreads = 256;
+constexpr int kScanWarps = kScanThreads / 32;
+constexpr int kPickThreads = 1024;
+constexpr int kPickWarps = kPickThreads / 32;
+constexpr int kPickCap = 1024;    // keys a prompt's selection may keep
+constexpr int kPickLists = 4096;  // lists whose places fit into shared memory beside them
+
+struct ChunkStats {
+  double sum;  // of exp(x - max)
+  float max;   // -inf: no logit; NaN: bad input
+  int32_t count;
+};
 
 struct BeamArgs {
   const void *logits;
@@ -26,156 +52,537 @@ struct BeamArgs {
   int32_t *parents, *tokens;
   uint8_t *next_finished;
   int32_t *status;
-  double *lse;     // [rows]; NaN: bad input
-  float *values;   // [rows][n_out] best logits, falling
-  int32_t *ids;    // [rows][n_out]; -1 behind the last
+  int32_t chunks;     // a row
+  int32_t cap;        // entries of a chunk's list
+  int32_t direct;     // too many lists to lay their entries end to end
+  double gap;
+  ChunkStats *stats;  // [rows][chunks]
+  float2 *lists;      // [rows][chunks][cap]: logit, token (bits)
 };
 
-// (a, i) stands before (b, j): the larger value, then the lower index.
-template <typename T>
-__device__ __forceinline__ bool before(T a, int64_t i, T b, int64_t j) {
-  return a > b || (a == b && i < j);
+// A row's terms exp(x - max) are each off by at most (3 |x - max| + 4) u relative (u = 2^-24:
+// the difference, its product with log2(e), the constant; ex2's 4 u); weighted by the
+// probabilities |x - max| averages to at most ln(vocab). Their fp32 sums add 14 u (runs of 8, 2,
+// a warp's tree). Two lse's differ by twice that.
+double gap_of(int32_t vocab) {
+  return 2.0 * (3.0 * log((double)std::max(vocab, 2)) + 20.0) * 5.9604644775390625e-8;
 }
 
-// The first of all threads' (v, id); id < 0 stands behind every other.
-template <typename T>
-__device__ void block_first(T &v, int64_t &id, T *sv, int64_t *si) {
-  const int t = threadIdx.x;
-  __syncthreads();
-  sv[t] = v;
-  si[t] = id;
-  __syncthreads();
-  for (int o = kThreads / 2; o > 0; o >>= 1) {
-    if (t < o && si[t + o] >= 0 && (si[t] < 0 || before(sv[t + o], si[t + o], sv[t], si[t]))) {
-      sv[t] = sv[t + o];
-      si[t] = si[t + o];
-    }
-    __syncthreads();
+template <typename T> struct Vec16;  // the values of 16 bytes
+template <> struct Vec16<float> {
+  static constexpr int kN = 4;
+  static __device__ __forceinline__ void get(uint4 v, float *x) {
+    x[0] = __uint_as_float(v.x);
+    x[1] = __uint_as_float(v.y);
+    x[2] = __uint_as_float(v.z);
+    x[3] = __uint_as_float(v.w);
   }
-  v = sv[0];
-  id = si[0];
+};
+template <> struct Vec16<__nv_bfloat16> {
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ void get(uint4 v, float *x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Vec16<__half> {
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ void get(uint4 v, float *x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+};
+
+// Logits are read once: past L1.
+__device__ __forceinline__ uint4 load_once(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// Order-preserving key with -0 folded onto +0.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t b = x == 0.f ? 0u : __float_as_uint(x);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_row_kernel(BeamArgs a) {
-  __shared__ double sd[kThreads];
-  __shared__ float sv[kThreads];
-  __shared__ int64_t si[kThreads];
-  const int row = blockIdx.x, t = threadIdx.x;
-  const int b = row / a.beams, i = row % a.beams;
+__device__ __forceinline__ const T *row_of(const BeamArgs &a, int row) {
+  return static_cast<const T *>(a.logits) + (row / a.beams) * a.batch_stride +
+         (row % a.beams) * a.beam_stride;
+}
+// 16-byte pieces of a row: piece v holds the elements v * kN - lead + 0 .. kN - 1 of it.
+template <typename T>
+__device__ __forceinline__ int lead_of(const T *x) {
+  return (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+}
+
+// The k best of the n logits in `x` (shared memory, in the order of their indexes, the first of
+// which is e0; at least k above -inf), ties to the lower index, in any order into `list`. The k-th
+// best value is found by bisection over the keys, bit by bit; then all above it are taken and, of
+// those equal to it, the first ones. All threads of the block call; returns k.
+__device__ __noinline__ int exact_list(const float *x, int n, int e0, int k, float2 *list) {
+  __shared__ int s_warp[kScanWarps], s_taken;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t kstar = 0;
+  for (int bit = 31; bit >= 0; bit--) {
+    const uint32_t probe = kstar | 1u << bit;
+    __syncthreads();
+    int c = 0;
+    for (int i = tid; i < n; i += kScanThreads) c += order_key(x[i]) >= probe ? 1 : 0;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) s_warp[warp] = c;
+    __syncthreads();
+    c = 0;
+    for (int w = 0; w < kScanWarps; w++) c += s_warp[w];
+    if (c >= k) kstar = probe;
+  }
+  if (tid == 0) s_taken = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += kScanThreads)
+    if (order_key(x[i]) > kstar) list[atomicAdd(&s_taken, 1)] = make_float2(x[i], __int_as_float(e0 + i));
+  __syncthreads();
+  int taken = s_taken;  // below k
+  for (int i0 = 0; i0 < n && taken < k; i0 += kScanThreads) {
+    const bool eq = i0 + tid < n && order_key(x[i0 + tid]) == kstar;
+    const unsigned m = __ballot_sync(0xffffffffu, eq);
+    __syncthreads();
+    if (lane == 0) s_warp[warp] = __popc(m);
+    __syncthreads();
+    int at = taken + __popc(m & ((1u << lane) - 1u)), all = 0;
+    for (int w = 0; w < kScanWarps; w++) {
+      if (w < warp) at += s_warp[w];
+      all += s_warp[w];
+    }
+    if (eq && at < k) list[at] = make_float2(x[i0 + tid], __int_as_float(e0 + i0 + tid));
+    taken = min(k, taken + all);
+  }
+  return k;
+}
+
+// NV pieces a thread: NV * kN logits in registers.
+template <typename T, int NV>
+__global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+  constexpr int kN = Vec16<T>::kN, kE = NV * kN;
+  __shared__ float s_max[kScanWarps], s_sum[kScanWarps];
+  __shared__ uint32_t s_bound[kScanWarps];
+  __shared__ int s_count;
+  __shared__ float s_x[kE * kScanThreads];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  ChunkStats *stats = a.stats + blockIdx.x;
+  float2 *list = a.lists + (int64_t)blockIdx.x * a.cap;
   const float score = a.scores[row];
-  const bool skip = score == -INFINITY || (a.finished && a.finished[row]);
-  const T *x = static_cast<const T *>(a.logits) + b * a.batch_stride + i * a.beam_stride;
-  float *values = a.values + (int64_t)row * a.n_out;
-  int32_t *ids = a.ids + (int64_t)row * a.n_out;
-  if (skip) {
-    for (int j = t; j < a.n_out; j += kThreads) ids[j] = -1;
-    if (t == 0) a.lse[row] = 0;
+  if (score == -INFINITY || (a.finished && a.finished[row])) {
+    if (tid == 0) *stats = {0.0, -INFINITY, 0};
     return;
   }
-  float m = -INFINITY;
-  bool bad = false;
-  for (int v = t; v < a.vocab; v += kThreads) {
-    const float f = to_f32(x[v]);
-    bad |= !(f < INFINITY);
-    m = fmaxf(m, f);
+  const T *x0 = row_of<T>(a, row);
+  const int lead = lead_of(x0);
+  const T *base = x0 - lead;
+  const int pieces = (int)(((int64_t)lead + a.vocab + kN - 1) / kN);
+  const int v0 = (int)((int64_t)chunk * pieces / a.chunks);
+  const int v1 = (int)((int64_t)(chunk + 1) * pieces / a.chunks);
+  float x[kE];
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const int v = v0 + j * kScanThreads + tid;
+    const int64_t e = (int64_t)v * kN - lead;  // the piece's first element
+    if (v < v1 && e >= 0 && e + kN <= a.vocab) {
+      Vec16<T>::get(load_once(base + (int64_t)v * kN), x + j * kN);
+    } else {  // outside, or a ragged end
+#pragma unroll
+      for (int i = 0; i < kN; i++)
+        x[j * kN + i] =
+            v < v1 && e + i >= 0 && e + i < a.vocab ? to_f32(x0[e + i]) : -INFINITY;
+    }
   }
-  bad = __syncthreads_or(bad);
-  int64_t id = t;
-  block_first(m, id, sv, si);
-  double s = 0;
-  if (m > -INFINITY)
-    for (int v = t; v < a.vocab; v += kThreads) s += exp((double)to_f32(x[v]) - (double)m);
-  sd[t] = s;
-  __syncthreads();
-  for (int o = kThreads / 2; o > 0; o >>= 1) {
-    if (t < o) sd[t] += sd[t + o];
-    __syncthreads();
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < kE; i++) top = max_nan(top, x[i]);
+  const bool bad = !(top < INFINITY);
+  // The warp's maximum and its ceil(n_out / 8)-th best thread maximum.
+  const uint32_t key = bad ? 0u : order_key(top);
+  uint32_t rest = key, kth = 0;
+  const uint32_t best = __reduce_max_sync(0xffffffffu, key);
+  for (int left = (a.n_out + kScanWarps - 1) / kScanWarps; left > 0;) {
+    kth = __reduce_max_sync(0xffffffffu, rest);
+    const unsigned eq = __ballot_sync(0xffffffffu, rest == kth);
+    left -= __popc(eq);
+    if (rest == kth) rest = 0;
+    if (kth == 0) break;
   }
-  if (t == 0) a.lse[row] = bad ? (double)NAN : (double)m + log(sd[0]);
-  float pv = INFINITY;
-  int64_t pi = -1;
-  for (int j = 0; j < a.n_out; j++) {
-    float best = -INFINITY;
-    int64_t at = -1;
-    if (!bad && pi < INT32_MAX) {
-      for (int v = t; v < a.vocab; v += kThreads) {
-        const float f = to_f32(x[v]);
-        if (f > -INFINITY && before(pv, pi, f, (int64_t)v) &&
-            (at < 0 || before(f, (int64_t)v, best, at))) {
-          best = f;
-          at = v;
-        }
+  const float wmax = best ? key_value(best) : -INFINITY;
+  // The sum relative to the warp's maximum.
+  float2 sum[2] = {};
+  if (wmax > -INFINITY) {
+    constexpr float kLog2e = 1.4426950408889634f;
+#pragma unroll
+    for (int i = 0; i < kE; i += 2) {
+      const float2 d = make_float2(x[i] - wmax, x[i + 1] - wmax);
+      const float2 e = make_float2(ex2_fast(d.x * kLog2e), ex2_fast(d.y * kLog2e));
+      sum[(i >> 1) & 1].x += e.x;
+      sum[(i >> 1) & 1].y += e.y;
+    }
+  }
+  float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) {
+    s_max[warp] = wmax;
+    s_sum[warp] = total;
+    s_bound[warp] = kth;
+  }
+  if (tid == 0) s_count = 0;
+  const bool any_bad = __syncthreads_or(bad);
+  if (any_bad) {
+    if (tid == 0) *stats = {0.0, NAN, 0};
+    return;
+  }
+  uint32_t bound = s_bound[0];
+  float cmax = s_max[0];
+#pragma unroll
+  for (int w = 1; w < kScanWarps; w++) {
+    bound = min(bound, s_bound[w]);
+    cmax = fmaxf(cmax, s_max[w]);
+  }
+  if (cmax == -INFINITY) {
+    if (tid == 0) *stats = {0.0, -INFINITY, 0};
+    return;
+  }
+  // Candidates: no smaller than the bound, above -inf.
+  const float least = bound <= order_key(-INFINITY) ? -3.402823466e38f : key_value(bound);
+  auto element = [&](int j, int i) { return (v0 + j * kScanThreads + tid) * kN - lead + i; };
+  if (top >= least) {
+#pragma unroll
+    for (int i = 0; i < kE; i++)
+      if (x[i] >= least) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < a.cap) list[at] = make_float2(x[i], __int_as_float(element(i / kN, i % kN)));
       }
-    }
-    block_first(best, at, sv, si);
-    if (t == 0) {
-      values[j] = best;
-      ids[j] = (int32_t)at;
-    }
-    pv = best;
-    pi = at < 0 ? INT32_MAX : at;
+  }
+  __syncthreads();
+  int count = s_count;
+  if (count > a.cap) {  // block-uniform
+#pragma unroll
+    for (int i = 0; i < kE; i++)
+      s_x[((i / kN) * kScanThreads + tid) * kN + i % kN] = x[i];
+    count = exact_list(s_x, kE * kScanThreads, v0 * kN - lead, a.n_out, list);
+  }
+  if (warp == 0) {
+    double t = 0;
+    if (lane < kScanWarps && s_max[lane] > -INFINITY)
+      t = (double)s_sum[lane] * exp((double)s_max[lane] - (double)cmax);
+    t = warp_sum(t);
+    if (lane == 0) *stats = {t, cmax, count};
   }
 }
 
-__global__ void __launch_bounds__(kThreads) beam_pick_kernel(BeamArgs a) {
-  __shared__ double sv[kThreads];
-  __shared__ int64_t si[kThreads];
-  const int b = blockIdx.x, t = threadIdx.x;
-  const int64_t row0 = (int64_t)b * a.beams;
+// A candidate: its key, its place (beam, then token), its logit.
+struct Cand {
+  double key;
+  float x;
+  int32_t beam, token;
+};
+// Within a beam the logits decide (their keys could round to the same), between beams the keys;
+// ties go to the lower beam, then token.
+__device__ __forceinline__ bool stands_before(const Cand &p, const Cand &q) {
+  if (p.beam == q.beam) return p.x > q.x || (p.x == q.x && p.token < q.token);
+  return p.key > q.key || (p.key == q.key && p.beam < q.beam);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid_constant__ BeamArgs a) {
+  __shared__ double s_lse[TABBY_BEAM_MAX], s_score[TABBY_BEAM_MAX];
+  __shared__ double s_bound[kPickWarps];
+  __shared__ Cand s_cand[kPickCap];
+  __shared__ int16_t s_order[kPickCap];
+  __shared__ float s_rowmax[TABBY_BEAM_MAX];
+  __shared__ uint8_t s_done[TABBY_BEAM_MAX], s_again[TABBY_BEAM_MAX];
+  __shared__ int s_count;
+  extern __shared__ int s_first[];  // [lists + 1] places of the lists' entries laid end to end
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row0 = b * a.beams, lists = a.beams * a.chunks;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const ChunkStats *stats = a.stats + (int64_t)row0 * a.chunks;
+  // Log-sum-exps, a warp a beam.
   bool bad = false;
-  for (int i = t; i < a.beams; i += kThreads) {
-    const float s = a.scores[row0 + i];
-    bad |= !(s < INFINITY) || isnan(a.lse[row0 + i]);
+  for (int i = warp; i < a.beams; i += kPickWarps) {
+    const float score = a.scores[row0 + i];
+    const bool done = a.finished && a.finished[row0 + i] && score != -INFINITY;
+    float m = -INFINITY;
+    for (int c = lane; c < a.chunks; c += 32) {
+      const float y = stats[i * a.chunks + c].max;
+      bad |= isnan(y);
+      m = fmaxf(m, y);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    double sum = 0;
+    for (int c = lane; c < a.chunks; c += 32) {
+      const ChunkStats s = stats[i * a.chunks + c];
+      if (s.max > -INFINITY) sum += s.sum * exp((double)s.max - (double)m);
+    }
+    sum = warp_sum(sum);
+    bad |= !(score < INFINITY);
+    if (lane == 0) {
+      s_rowmax[i] = m;
+      s_lse[i] = m > -INFINITY ? (double)m + log(sum) : 0.0;
+      s_score[i] = score;
+      s_done[i] = done;
+      s_again[i] = 0;
+    }
   }
   bad = __syncthreads_or(bad);
-  double pv = INFINITY;
-  int64_t pi = -1;
-  bool none = bad;
-  for (int j = 0; j < a.n_out; j++) {
-    double best = -INFINITY;
-    int64_t at = -1;
-    if (!none) {
-      for (int c = t; c < a.beams * a.n_out; c += kThreads) {
-        const int i = c / a.n_out, e = c % a.n_out;
-        const int64_t row = row0 + i;
-        const float score = a.scores[row];
-        if (score == -INFINITY) continue;
-        double key;
-        int64_t id;
-        if (a.finished && a.finished[row]) {
-          if (e != 0) continue;
-          key = score;
-          id = (int64_t)i * a.vocab + a.eos;
-        } else {
-          const int32_t v = a.ids[row * a.n_out + e];
-          if (v < 0) continue;
-          key = (double)score + ((double)a.values[row * a.n_out + e] - a.lse[row]);
-          id = (int64_t)i * a.vocab + v;
-        }
-        if (before(pv, pi, key, id) && (at < 0 || before(key, id, best, at))) {
-          best = key;
-          at = id;
-        }
+  auto write = [&](int j, bool none, const Cand &c) {
+    const int64_t o = (int64_t)b * a.n_out + j;
+    a.next_scores[o] = none ? -INFINITY : (float)c.key;
+    a.parents[o] = none ? -1 : c.beam;
+    a.tokens[o] = none ? -1 : c.token;
+    if (a.next_finished) a.next_finished[o] = none || c.token == a.eos || s_done[c.beam] ? 1 : 0;
+  };
+  if (tid == 0) a.status[b] = bad ? TABBY_EINPUT : TABBY_OK;
+  if (bad) {
+    for (int j = tid; j < a.n_out; j += kPickThreads) write(j, true, Cand());
+    return;
+  }
+  // The lists' entries laid end to end (or every place of every list), then one a finished beam.
+  if (!a.direct && warp == 0) {
+    int base = 0;
+    for (int l0 = 0; l0 < lists; l0 += 32) {
+      const int n = l0 + lane < lists ? stats[l0 + lane].count : 0;
+      int end = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += y;
+      }
+      if (l0 + lane < lists) s_first[l0 + lane] = base + end - n;
+      base += __shfl_sync(0xffffffffu, end, 31);
+    }
+    if (lane == 0) s_first[lists] = base;
+  }
+  __syncthreads();
+  const int listed = a.direct ? lists * a.cap : s_first[lists], all = listed + a.beams;
+  auto get = [&](int f, Cand &c) {  // false: no candidate
+    if (f >= listed) {
+      c.beam = f - listed;
+      c.token = a.eos;
+      c.x = 0.f;
+      c.key = s_score[c.beam];
+      return s_done[c.beam] != 0;
+    }
+    int lo = 0, at = 0;
+    if (a.direct) {
+      lo = f / a.cap;
+      at = f - lo * a.cap;
+      if (at >= stats[lo].count) return false;
+    } else {  // the last list that begins at or before f
+      for (int hi = lists; hi - lo > 1;) {
+        const int mid = (lo + hi) >> 1;
+        if (s_first[mid] <= f) lo = mid;
+        else hi = mid;
+      }
+      at = f - s_first[lo];
+    }
+    const float2 y = a.lists[((int64_t)row0 * a.chunks + lo) * a.cap + at];
+    c.beam = lo / a.chunks;
+    c.token = __float_as_int(y.y);
+    c.x = y.x;
+    c.key = s_score[c.beam] + ((double)y.x - s_lse[c.beam]);
+    return true;
+  };
+  // A bound on the n_out-th best key, as in the scan: entry f goes to warp f mod 32, so that
+  // every warp sees all beams.
+  const int step = kPickThreads, place = lane * kPickWarps + warp;
+  double top = -INFINITY;
+  for (int f = place; f < all; f += step) {
+    Cand c;
+    if (get(f, c)) top = fmax(top, c.key);
+  }
+  {
+    double rest = top, kth = -INFINITY;
+    for (int left = (a.n_out + kPickWarps - 1) / kPickWarps; left > 0;) {
+      kth = rest;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) kth = fmax(kth, __shfl_xor_sync(0xffffffffu, kth, o));
+      if (kth == -INFINITY) break;
+      left -= __popc(__ballot_sync(0xffffffffu, rest == kth));
+      if (rest == kth) rest = -INFINITY;
+    }
+    if (lane == 0) s_bound[warp] = kth;
+  }
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  double bound = s_bound[0];
+  for (int w = 1; w < kPickWarps; w++) bound = fmin(bound, s_bound[w]);
+  const double least = bound - 2 * a.gap;  // what more exact keys might still bring up
+  for (int f = place; f < all; f += step) {
+    Cand c;
+    if (get(f, c) && c.key >= least) {
+      const int at = atomicAdd(&s_count, 1);
+      if (at < kPickCap) s_cand[at] = c;
+    }
+  }
+  __syncthreads();
+  // The lse of the marked beams in 64 bits, from all their logits.
+  auto refine = [&]() {
+    for (int i = 0; i < a.beams; i++) {
+      if (!s_again[i]) continue;
+      const T *x = row_of<T>(a, row0 + i);
+      const double m = s_rowmax[i];
+      double sum = 0;
+      for (int v = tid; v < a.vocab; v += kPickThreads) sum += exp((double)to_f32(x[v]) - m);
+      sum = warp_sum(sum);
+      __syncthreads();
+      if (lane == 0) s_bound[warp] = sum;
+      __syncthreads();
+      if (warp == 0) {
+        sum = warp_sum(s_bound[lane]);
+        if (lane == 0) s_lse[i] = m + log(sum);
       }
     }
-    block_first(best, at, sv, si);
-    none |= at < 0;
-    if (t == 0) {
-      const int64_t o = (int64_t)b * a.n_out + j;
-      const int32_t parent = none ? -1 : (int32_t)(at / a.vocab);
-      const int32_t token = none ? -1 : (int32_t)(at % a.vocab);
-      a.next_scores[o] = none ? -INFINITY : (float)best;
-      a.parents[o] = parent;
-      a.tokens[o] = token;
-      if (a.next_finished)
-        a.next_finished[o] =
-            none || token == a.eos || (a.finished && a.finished[row0 + parent]) ? 1 : 0;
+    __syncthreads();
+  };
+  const bool many = s_count > kPickCap;
+  if (many) {
+    // Too many for the table, by ties: with all keys exact, the best one after the other.
+    __syncthreads();
+    if (tid == 0) s_count = 0;
+    for (int i = tid; i < a.beams; i += kPickThreads)
+      s_again[i] = !s_done[i] && s_rowmax[i] > -INFINITY;
+    __syncthreads();
+    refine();
+    __shared__ Cand s_best[kPickWarps], s_last;
+    Cand last;
+    last.key = INFINITY;
+    last.x = INFINITY;
+    last.beam = -1;
+    last.token = -1;
+    for (int j = 0; j < a.n_out; j++) {
+      Cand best;
+      best.beam = -1;
+      for (int f = place; f < all; f += step) {
+        Cand c;
+        if (get(f, c) && (last.beam < 0 || stands_before(last, c)) &&
+            (best.beam < 0 || stands_before(c, best)))
+          best = c;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        Cand c;
+        c.key = __shfl_xor_sync(0xffffffffu, best.key, o);
+        c.x = __shfl_xor_sync(0xffffffffu, best.x, o);
+        c.beam = __shfl_xor_sync(0xffffffffu, best.beam, o);
+        c.token = __shfl_xor_sync(0xffffffffu, best.token, o);
+        if (c.beam >= 0 && (best.beam < 0 || stands_before(c, best))) best = c;
+      }
+      if (lane == 0) s_best[warp] = best;
+      __syncthreads();
+      if (tid == 0) {
+        best = s_best[0];
+        for (int w = 1; w < kPickWarps; w++)
+          if (s_best[w].beam >= 0 && (best.beam < 0 || stands_before(s_best[w], best)))
+            best = s_best[w];
+        s_last = best;
+        if (best.beam >= 0) s_cand[s_count++] = best;
+      }
+      __syncthreads();
+      last = s_last;
+      if (last.beam < 0) break;
     }
-    pv = best;
-    pi = at;
+    __syncthreads();
   }
-  if (t == 0) a.status[b] = bad ? TABBY_EINPUT : TABBY_OK;
+  const int n = s_count;
+  auto rank = [&]() {  // s_order[j]: the candidate of rank j
+    for (int i = tid; i < n; i += kPickThreads) {
+      const Cand c = s_cand[i];
+      int r = 0;
+      for (int k = 0; k < n; k++) r += stands_before(s_cand[k], c) ? 1 : 0;
+      s_order[r] = (int16_t)i;
+    }
+    __syncthreads();
+  };
+  rank();
+  // Neighbours of different beams that are too close to be told apart by fp32 sums, down to
+  // those that are as close to the last one chosen.
+  bool close = false;
+  const double lowest = n > 0 ? s_cand[s_order[min(n, a.n_out) - 1]].key - a.gap : 0.0;
+  for (int j = tid; !many && j < n - 1; j += kPickThreads) {
+    const Cand p = s_cand[s_order[j]], q = s_cand[s_order[j + 1]];
+    if (q.key >= lowest && p.beam != q.beam && p.key - q.key < a.gap) {
+      if (!s_done[p.beam]) s_again[p.beam] = 1, close = true;
+      if (!s_done[q.beam]) s_again[q.beam] = 1, close = true;
+    }
+  }
+  if (__syncthreads_or(close)) {
+    refine();
+    for (int i = tid; i < n; i += kPickThreads)
+      if (const int k = s_cand[i].beam; s_again[k])
+        s_cand[i].key = s_score[k] + ((double)s_cand[i].x - s_lse[k]);
+    __syncthreads();
+    rank();
+  }
+  for (int j = tid; j < a.n_out; j += kPickThreads)
+    write(j, j >= n, j < n ? s_cand[s_order[j]] : Cand());
+}
+
+// Chunks of a row: at most 256 threads' worth of pieces each.
+struct ScanPlan {
+  int nv;      // pieces a thread
+  int chunks;  // a row
+  int cap;     // entries of a list
+};
+ScanPlan scan_plan(int64_t rows, int32_t vocab, int32_t dtype, int32_t n_out) {
+  const int n = dtype == TABBY_F32 ? 4 : 8;
+  const int64_t pieces = ((int64_t)vocab + 2 * n - 2) / n;  // at most, however a row is aligned
+  auto chunks = [&](int nv) {
+    return (int)((pieces + (int64_t)nv * kScanThreads - 1) / ((int64_t)nv * kScanThreads));
+  };
+  ScanPlan p;
+  p.nv = 32 / n;
+  if (rows * chunks(p.nv) < 148) p.nv = 16 / n;  // few rows: half the chunk, twice the CTAs
+  p.chunks = chunks(p.nv);
+  p.cap = std::max(128, 4 * n_out);
+  return p;
+}
+
+template <typename T>
+cudaError_t launch_beam(const BeamArgs &a, int nv, cudaStream_t q) {
+  constexpr int kN = Vec16<T>::kN;
+  const dim3 grid((unsigned)a.batch * (unsigned)a.beams * (unsigned)a.chunks);
+  cudaError_t err =
+      nv == 32 / kN ? launch_pdl(beam_scan_kernel<T, 32 / kN>, grid, kScanThreads, 0, q, a)
+                    : launch_pdl(beam_scan_kernel<T, 16 / kN>, grid, kScanThreads, 0, q, a);
+  if (err != cudaSuccess) return err;
+  return launch_pdl(beam_pick_kernel<T>, dim3((unsigned)a.batch), kPickThreads,
+                    a.direct ? 0 : ((size_t)a.beams * a.chunks + 1) * sizeof(int), q, a);
 }
 
 int check_sizes(int32_t batch, int32_t beams, int32_t vocab, int32_t n_out) {
@@ -188,8 +595,11 @@ int check_sizes(int32_t batch, int32_t beams, int32_t vocab, int32_t n_out) {
   if (n_out < 1 || n_out > TABBY_BEAM_MAX_OUT)
     return decode_fail(TABBY_EINVAL, "beam_step: n_out must be in [1, %d], got %d",
                        TABBY_BEAM_MAX_OUT, n_out);
-  if ((int64_t)batch * beams > (1 << 22))
-    return decode_fail(TABBY_EINVAL, "beam_step: batch * beams must be at most 2^22");
+  if ((int64_t)beams * vocab > INT32_MAX)
+    return decode_fail(TABBY_EINVAL, "beam_step: beams * vocab must be below 2^31");
+  for (int32_t dtype : {TABBY_F32, TABBY_BF16, TABBY_F16})
+    if ((int64_t)batch * beams > INT32_MAX / scan_plan((int64_t)batch * beams, vocab, dtype, n_out).chunks)
+      return decode_fail(TABBY_EINVAL, "beam_step: batch * beams * vocab is too large");
   return TABBY_OK;
 }
 
@@ -204,8 +614,13 @@ int tabby_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab, int3
   const int st = check_sizes(batch, beams, vocab, n_out);
   if (st) return st;
   if (!bytes) return decode_fail(TABBY_EINVAL, "beam_step: bytes is NULL");
-  const size_t rows = (size_t)batch * beams;
-  *bytes = rows * 8 + rows * n_out * 8;
+  // The most that any type's plan takes.
+  *bytes = 0;
+  for (int32_t dtype : {TABBY_F32, TABBY_BF16, TABBY_F16}) {
+    const ScanPlan p = scan_plan((int64_t)batch * beams, vocab, dtype, n_out);
+    *bytes = std::max(*bytes, (size_t)batch * beams * p.chunks *
+                                  (sizeof(ChunkStats) + p.cap * sizeof(float2)));
+  }
   return TABBY_OK;
 }
 
@@ -256,18 +671,17 @@ int tabby_beam_step_async(int32_t device, const void *d_logits, int32_t dtype,
   a.next_finished = d_next_finished;
   a.status = d_status;
   const size_t rows = (size_t)batch * beams;
-  a.lse = static_cast<double *>(d_workspace);
-  a.values = reinterpret_cast<float *>(a.lse + rows);
-  a.ids = reinterpret_cast<int32_t *>(a.values + rows * n_out);
+  const ScanPlan plan = scan_plan((int64_t)rows, vocab, dtype, n_out);
+  a.chunks = plan.chunks;
+  a.cap = plan.cap;
+  a.direct = (int64_t)beams * plan.chunks > kPickLists;
+  a.gap = gap_of(vocab);
+  a.stats = static_cast<ChunkStats *>(d_workspace);
+  a.lists = reinterpret_cast<float2 *>(a.stats + rows * plan.chunks);
   cudaStream_t q = static_cast<cudaStream_t>(stream);
-  if (dtype == TABBY_F32)
-    beam_row_kernel<float><<<(unsigned)rows, kThreads, 0, q>>>(a);
-  else if (dtype == TABBY_BF16)
-    beam_row_kernel<__nv_bfloat16><<<(unsigned)rows, kThreads, 0, q>>>(a);
-  else
-    beam_row_kernel<__half><<<(unsigned)rows, kThreads, 0, q>>>(a);
-  beam_pick_kernel<<<(unsigned)batch, kThreads, 0, q>>>(a);
-  const cudaError_t err = cudaGetLastError();
+  const cudaError_t err = dtype == TABBY_F32    ? launch_beam<float>(a, plan.nv, q)
+                          : dtype == TABBY_BF16 ? launch_beam<__nv_bfloat16>(a, plan.nv, q)
+                                                : launch_beam<__half>(a, plan.nv, q);
   if (err != cudaSuccess) return decode_cuda_fail(err, "beam_step launch");
   return TABBY_OK;
 }
