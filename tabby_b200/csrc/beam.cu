@@ -17,7 +17,8 @@
 // The sums of a chunk are in fp32, so a lse is off by up to gap / 2 (gap_of below), and keys of
 // different beams that are closer than the gap might be out of order. Such pairs are rare; where
 // the sorted result has one, the lse of the beams in it is computed again in 64 bits from all
-// their logits (the rows are read once more) and the listed keys are sorted again.
+// their logits (the rows are read once more, by a cluster of CTAs) and the listed keys are sorted
+// again.
 #include <math.h>
 
 #include <algorithm>
@@ -32,14 +33,15 @@ constexpr int kScanThreads = 256;
 constexpr int kScanWarps = kScanThreads / 32;
 constexpr int kPickThreads = 1024;
 constexpr int kPickWarps = kPickThreads / 32;
-constexpr int kPickCap = 1024;    // keys a prompt's selection may keep
-constexpr int kPickLists = 4096;  // lists whose places fit into shared memory beside them
+constexpr int kMaxHelpers = 8;
+constexpr int kPickCap = 1024;  // keys a prompt's selection may keep
 
 struct ChunkStats {
   double sum;  // of exp(x - max)
   float max;   // -inf: no logit; NaN: bad input
   int32_t count;
 };
+constexpr int kPickTight = 256;  // more keys than this are worth a tighter bound
 
 struct BeamArgs {
   const void *logits;
@@ -52,9 +54,9 @@ struct BeamArgs {
   int32_t *parents, *tokens;
   uint8_t *next_finished;
   int32_t *status;
+  int32_t helpers;    // CTAs a prompt of the pick: a cluster
   int32_t chunks;     // a row
   int32_t cap;        // entries of a chunk's list
-  int32_t direct;     // too many lists to lay their entries end to end
   double gap;
   ChunkStats *stats;  // [rows][chunks]
   float2 *lists;      // [rows][chunks][cap]: logit, token (bits)
@@ -109,12 +111,6 @@ __device__ __forceinline__ uint4 load_once(const void *p) {
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
-}
-// Maximum that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
 }
 // Order-preserving key with -0 folded onto +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -210,22 +206,36 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   const int v0 = (int)((int64_t)chunk * pieces / a.chunks);
   const int v1 = (int)((int64_t)(chunk + 1) * pieces / a.chunks);
   float x[kE];
+  if ((int64_t)v0 * kN >= lead && (int64_t)v1 * kN - lead <= a.vocab) {  // whole pieces only
+    const T *p = base + (int64_t)(v0 + tid) * kN;
 #pragma unroll
-  for (int j = 0; j < NV; j++) {
-    const int v = v0 + j * kScanThreads + tid;
-    const int64_t e = (int64_t)v * kN - lead;  // the piece's first element
-    if (v < v1 && e >= 0 && e + kN <= a.vocab) {
-      Vec16<T>::get(load_once(base + (int64_t)v * kN), x + j * kN);
-    } else {  // outside, or a ragged end
+    for (int j = 0; j < NV; j++) {
+      if (j * kScanThreads + tid < v1 - v0) {
+        Vec16<T>::get(load_once(p + j * kScanThreads * kN), x + j * kN);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kN; i++) x[j * kN + i] = -INFINITY;
+      }
+    }
+  } else {  // a row's ragged ends
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int v = v0 + j * kScanThreads + tid;
+      const int64_t e = (int64_t)v * kN - lead;  // the piece's first element
 #pragma unroll
       for (int i = 0; i < kN; i++)
         x[j * kN + i] =
             v < v1 && e + i >= 0 && e + i < a.vocab ? to_f32(x0[e + i]) : -INFINITY;
     }
   }
-  float top = x[0];
+  float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-  for (int i = 1; i < kE; i++) top = max_nan(top, x[i]);
+  for (int i = 4; i < kE - 4; i += 8)
+#pragma unroll
+    for (int k = 0; k < 4; k++) mx[k] = max3_nan(mx[k], x[i + 2 * k], x[i + 2 * k + 1]);
+  const float top =
+      max3_nan(max3_nan(mx[0], mx[1], x[kE - 4]), max3_nan(mx[2], mx[3], x[kE - 3]),
+               max3_nan(x[kE - 2], x[kE - 1], x[0]));
   const bool bad = !(top < INFINITY);
   // The warp's maximum and its ceil(n_out / 8)-th best thread maximum.
   const uint32_t key = bad ? 0u : order_key(top);
@@ -243,12 +253,11 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   float2 sum[2] = {};
   if (wmax > -INFINITY) {
     constexpr float kLog2e = 1.4426950408889634f;
+    const float2 m2 = make_float2(-wmax, -wmax), l2 = make_float2(kLog2e, kLog2e);
 #pragma unroll
     for (int i = 0; i < kE; i += 2) {
-      const float2 d = make_float2(x[i] - wmax, x[i + 1] - wmax);
-      const float2 e = make_float2(ex2_fast(d.x * kLog2e), ex2_fast(d.y * kLog2e));
-      sum[(i >> 1) & 1].x += e.x;
-      sum[(i >> 1) & 1].y += e.y;
+      const float2 t = mul2(add2(make_float2(x[i], x[i + 1]), m2), l2);
+      sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], make_float2(ex2_fast(t.x), ex2_fast(t.y)));
     }
   }
   float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -317,20 +326,71 @@ __device__ __forceinline__ bool stands_before(const Cand &p, const Cand &q) {
   return p.key > q.key || (p.key == q.key && p.beam < q.beam);
 }
 
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of the first CTA's copy of a shared variable, for the cluster's other CTAs.
+__device__ __forceinline__ uint32_t in_first_cta(const void *p) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr(p)));
+  return r;
+}
+__device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid_constant__ BeamArgs a) {
   __shared__ double s_lse[TABBY_BEAM_MAX], s_score[TABBY_BEAM_MAX];
   __shared__ double s_bound[kPickWarps];
   __shared__ Cand s_cand[kPickCap];
   __shared__ int16_t s_order[kPickCap];
+  __shared__ int s_rank[kPickCap];
   __shared__ float s_rowmax[TABBY_BEAM_MAX];
-  __shared__ uint8_t s_done[TABBY_BEAM_MAX], s_again[TABBY_BEAM_MAX];
+  __shared__ uint8_t s_done[TABBY_BEAM_MAX];
+  __shared__ uint32_t s_again[TABBY_BEAM_MAX], s_need;
+  __shared__ double s_part[kMaxHelpers][TABBY_BEAM_MAX];
   __shared__ int s_count;
-  extern __shared__ int s_first[];  // [lists + 1] places of the lists' entries laid end to end
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.x / a.helpers, helper = blockIdx.x - b * a.helpers, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row0 = b * a.beams, lists = a.beams * a.chunks;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const ChunkStats *stats = a.stats + (int64_t)row0 * a.chunks;
+  // This CTA's share of sum exp(x - m) over beam i's logits, in 64 bits.
+  auto share = [&](int i, float m, uint32_t to) {
+    const T *x = row_of<T>(a, row0 + i);
+    const int n = (a.vocab + a.helpers - 1) / a.helpers;
+    double sum = 0;
+    for (int v = helper * n + tid; v < min(a.vocab, (helper + 1) * n); v += kPickThreads)
+      sum += exp((double)to_f32(x[v]) - (double)m);
+    sum = warp_sum(sum);
+    __syncthreads();
+    if (lane == 0) s_bound[warp] = sum;
+    __syncthreads();
+    if (warp == 0) {
+      sum = warp_sum(s_bound[lane]);
+      if (lane == 0) store_cluster(to, sum);
+    }
+  };
+  if (helper > 0) {  // waits for the first CTA's word
+    cluster_arrive();
+    cluster_wait();
+    if (load_cluster(in_first_cta(&s_need)))
+      for (int i = 0; i < a.beams; i++)
+        if (load_cluster(in_first_cta(&s_again[i])))
+          share(i, __uint_as_float(load_cluster(in_first_cta(&s_rowmax[i]))),
+                in_first_cta(&s_part[helper][i]));
+    cluster_arrive();
+    cluster_wait();
+    return;
+  }
   // Log-sum-exps, a warp a beam.
   bool bad = false;
   for (int i = warp; i < a.beams; i += kPickWarps) {
@@ -370,103 +430,96 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
   if (tid == 0) a.status[b] = bad ? TABBY_EINPUT : TABBY_OK;
   if (bad) {
     for (int j = tid; j < a.n_out; j += kPickThreads) write(j, true, Cand());
+    if (tid == 0) s_need = 0;
+    cluster_arrive();
+    cluster_wait();
+    cluster_arrive();
+    cluster_wait();  // the others have read the word
     return;
   }
-  // The lists' entries laid end to end (or every place of every list), then one a finished beam.
-  if (!a.direct && warp == 0) {
-    int base = 0;
-    for (int l0 = 0; l0 < lists; l0 += 32) {
-      const int n = l0 + lane < lists ? stats[l0 + lane].count : 0;
-      int end = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, end, o);
-        if (lane >= o) end += y;
-      }
-      if (l0 + lane < lists) s_first[l0 + lane] = base + end - n;
-      base += __shfl_sync(0xffffffffu, end, 31);
-    }
-    if (lane == 0) s_first[lists] = base;
-  }
-  __syncthreads();
-  const int listed = a.direct ? lists * a.cap : s_first[lists], all = listed + a.beams;
-  auto get = [&](int f, Cand &c) {  // false: no candidate
-    if (f >= listed) {
-      c.beam = f - listed;
-      c.token = a.eos;
-      c.x = 0.f;
-      c.key = s_score[c.beam];
-      return s_done[c.beam] != 0;
-    }
-    int lo = 0, at = 0;
-    if (a.direct) {
-      lo = f / a.cap;
-      at = f - lo * a.cap;
-      if (at >= stats[lo].count) return false;
-    } else {  // the last list that begins at or before f
-      for (int hi = lists; hi - lo > 1;) {
-        const int mid = (lo + hi) >> 1;
-        if (s_first[mid] <= f) lo = mid;
-        else hi = mid;
-      }
-      at = f - s_first[lo];
-    }
-    const float2 y = a.lists[((int64_t)row0 * a.chunks + lo) * a.cap + at];
-    c.beam = lo / a.chunks;
+  // Entry e of list l, a list's best key.
+  auto entry = [&](int l, int e) {
+    const float2 y = a.lists[((int64_t)row0 * a.chunks + l) * a.cap + e];
+    Cand c;
+    c.beam = l / a.chunks;
     c.token = __float_as_int(y.y);
     c.x = y.x;
     c.key = s_score[c.beam] + ((double)y.x - s_lse[c.beam]);
-    return true;
+    return c;
   };
-  // A bound on the n_out-th best key, as in the scan: entry f goes to warp f mod 32, so that
-  // every warp sees all beams.
-  const int step = kPickThreads, place = lane * kPickWarps + warp;
-  double top = -INFINITY;
-  for (int f = place; f < all; f += step) {
+  auto list_top = [&](int l) {
+    const int i = l / a.chunks;
+    const float m = stats[l].max;
+    return m > -INFINITY ? s_score[i] + ((double)m - s_lse[i]) : -INFINITY;
+  };
+  auto finished = [&](int i) {
     Cand c;
-    if (get(f, c)) top = fmax(top, c.key);
-  }
-  {
-    double rest = top, kth = -INFINITY;
-    for (int left = (a.n_out + kPickWarps - 1) / kPickWarps; left > 0;) {
-      kth = rest;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) kth = fmax(kth, __shfl_xor_sync(0xffffffffu, kth, o));
-      if (kth == -INFINITY) break;
-      left -= __popc(__ballot_sync(0xffffffffu, rest == kth));
-      if (rest == kth) rest = -INFINITY;
+    c.beam = i;
+    c.token = a.eos;
+    c.x = 0.f;
+    c.key = s_score[i];
+    return c;
+  };
+  // A bound below the n_out-th largest of the threads' values (-inf where there are fewer), so
+  // that at least n_out keys are no smaller: by bisection over the values rounded down to fp32.
+  auto bound_of = [&](double top) {
+    const uint32_t key = order_key(__double2float_rd(top));
+    uint32_t kth = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+      const uint32_t probe = kth | 1u << bit;
+      if (__syncthreads_count(key >= probe) >= a.n_out) kth = probe;
     }
-    if (lane == 0) s_bound[warp] = kth;
-  }
-  if (tid == 0) s_count = 0;
-  __syncthreads();
-  double bound = s_bound[0];
-  for (int w = 1; w < kPickWarps; w++) bound = fmin(bound, s_bound[w]);
-  const double least = bound - 2 * a.gap;  // what more exact keys might still bring up
-  for (int f = place; f < all; f += step) {
-    Cand c;
-    if (get(f, c) && c.key >= least) {
-      const int at = atomicAdd(&s_count, 1);
-      if (at < kPickCap) s_cand[at] = c;
-    }
-  }
-  __syncthreads();
-  // The lse of the marked beams in 64 bits, from all their logits.
-  auto refine = [&]() {
-    for (int i = 0; i < a.beams; i++) {
-      if (!s_again[i]) continue;
-      const T *x = row_of<T>(a, row0 + i);
-      const double m = s_rowmax[i];
-      double sum = 0;
-      for (int v = tid; v < a.vocab; v += kPickThreads) sum += exp((double)to_f32(x[v]) - m);
-      sum = warp_sum(sum);
-      __syncthreads();
-      if (lane == 0) s_bound[warp] = sum;
-      __syncthreads();
-      if (warp == 0) {
-        sum = warp_sum(s_bound[lane]);
-        if (lane == 0) s_lse[i] = m + log(sum);
+    return kth > order_key(-INFINITY) ? (double)key_value(kth) : -INFINITY;
+  };
+  auto keep = [&](const Cand &c, double least) {
+    if (c.key < least) return;
+    const int at = atomicAdd(&s_count, 1);
+    if (at < kPickCap) s_cand[at] = c;
+  };
+  // What is no smaller than a bound, less what more exact keys might bring up. Lists go round
+  // the warps, 32 at a time a warp, and only those whose best passes are read.
+  auto collect = [&](double bound) {
+    const double least = bound - 2 * a.gap;
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    for (int l0 = 0; l0 < lists; l0 += kPickThreads) {
+      const int l = l0 + lane * kPickWarps + warp;
+      const int count = l < lists ? stats[l].count : 0;
+      unsigned pass = __ballot_sync(0xffffffffu, count > 0 && list_top(l) >= least);
+      for (; pass; pass &= pass - 1) {
+        const int f = __ffs(pass) - 1, n = __shfl_sync(0xffffffffu, count, f);
+        for (int e = lane; e < n; e += 32) keep(entry(l0 + f * kPickWarps + warp, e), least);
       }
+    }
+    for (int i = tid; i < a.beams; i += kPickThreads)
+      if (s_done[i]) keep(finished(i), least);
+    __syncthreads();
+  };
+  // A bound from the lists' bests; where too much passes it, one from the entries.
+  double top = -INFINITY;
+  for (int l = tid; l < lists; l += kPickThreads) top = fmax(top, list_top(l));
+  collect(bound_of(top));
+  if (s_count > kPickTight) {
+    top = -INFINITY;
+    for (int u = warp; u < 4 * lists; u += kPickWarps)  // a quarter of a list
+      for (int e = (u & 3) * 32 + lane; e < stats[u >> 2].count; e += 128)
+        top = fmax(top, entry(u >> 2, e).key);
+    collect(bound_of(top));
+  }
+  // The lse of the marked beams in 64 bits, from all their logits, with the cluster's help.
+  auto refine = [&]() {
+    if (tid == 0) s_need = 1;
+    cluster_arrive();
+    cluster_wait();
+    for (int i = 0; i < a.beams; i++)
+      if (s_again[i]) share(i, s_rowmax[i], in_first_cta(&s_part[0][i]));
+    cluster_arrive();
+    cluster_wait();
+    for (int i = tid; i < a.beams; i += kPickThreads) {
+      if (!s_again[i]) continue;
+      double sum = 0;
+      for (int k = 0; k < a.helpers; k++) sum += s_part[k][i];
+      s_lse[i] = (double)s_rowmax[i] + log(sum);
     }
     __syncthreads();
   };
@@ -488,12 +541,15 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
     for (int j = 0; j < a.n_out; j++) {
       Cand best;
       best.beam = -1;
-      for (int f = place; f < all; f += step) {
-        Cand c;
-        if (get(f, c) && (last.beam < 0 || stands_before(last, c)) &&
+      auto consider = [&](const Cand &c) {
+        if ((last.beam < 0 || stands_before(last, c)) &&
             (best.beam < 0 || stands_before(c, best)))
           best = c;
-      }
+      };
+      for (int l = warp; l < lists; l += kPickWarps)
+        for (int e = lane; e < stats[l].count; e += 32) consider(entry(l, e));
+      for (int i = tid; i < a.beams; i += kPickThreads)
+        if (s_done[i]) consider(finished(i));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         Cand c;
@@ -520,13 +576,19 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
     __syncthreads();
   }
   const int n = s_count;
-  auto rank = [&]() {  // s_order[j]: the candidate of rank j
-    for (int i = tid; i < n; i += kPickThreads) {
-      const Cand c = s_cand[i];
+  auto rank = [&]() {  // s_order[j]: the candidate of rank j; a few threads a candidate
+    const int parts = max(1, kPickThreads / max(n, 1));
+    for (int i = tid; i < n; i += kPickThreads) s_rank[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n * parts; i += kPickThreads) {
+      const int p = i / n, me = i - p * n;
+      const Cand c = s_cand[me];
       int r = 0;
-      for (int k = 0; k < n; k++) r += stands_before(s_cand[k], c) ? 1 : 0;
-      s_order[r] = (int16_t)i;
+      for (int k = p; k < n; k += parts) r += stands_before(s_cand[k], c) ? 1 : 0;
+      if (r) atomicAdd(&s_rank[me], r);
     }
+    __syncthreads();
+    for (int i = tid; i < n; i += kPickThreads) s_order[s_rank[i]] = (int16_t)i;
     __syncthreads();
   };
   rank();
@@ -541,7 +603,8 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
       if (!s_done[q.beam]) s_again[q.beam] = 1, close = true;
     }
   }
-  if (__syncthreads_or(close)) {
+  const bool again = __syncthreads_or(close);
+  if (again) {
     refine();
     for (int i = tid; i < n; i += kPickThreads)
       if (const int k = s_cand[i].beam; s_again[k])
@@ -549,8 +612,18 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
     __syncthreads();
     rank();
   }
+  if (!again && !many) {
+    if (tid == 0) s_need = 0;
+    cluster_arrive();
+    cluster_wait();
+    cluster_arrive();
+  }
   for (int j = tid; j < a.n_out; j += kPickThreads)
     write(j, j >= n, j < n ? s_cand[s_order[j]] : Cand());
+  if (!again && !many) {
+    __syncwarp();
+    cluster_wait();  // the others have read the word
+  }
 }
 
 // Chunks of a row: at most 256 threads' worth of pieces each.
@@ -581,8 +654,18 @@ cudaError_t launch_beam(const BeamArgs &a, int nv, cudaStream_t q) {
       nv == 32 / kN ? launch_pdl(beam_scan_kernel<T, 32 / kN>, grid, kScanThreads, 0, q, a)
                     : launch_pdl(beam_scan_kernel<T, 16 / kN>, grid, kScanThreads, 0, q, a);
   if (err != cudaSuccess) return err;
-  return launch_pdl(beam_pick_kernel<T>, dim3((unsigned)a.batch), kPickThreads,
-                    a.direct ? 0 : ((size_t)a.beams * a.chunks + 1) * sizeof(int), q, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.batch * a.helpers));
+  cfg.blockDim = dim3(kPickThreads);
+  cfg.stream = q;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)a.helpers, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, beam_pick_kernel<T>, a);
 }
 
 int check_sizes(int32_t batch, int32_t beams, int32_t vocab, int32_t n_out) {
@@ -674,7 +757,9 @@ int tabby_beam_step_async(int32_t device, const void *d_logits, int32_t dtype,
   const ScanPlan plan = scan_plan((int64_t)rows, vocab, dtype, n_out);
   a.chunks = plan.chunks;
   a.cap = plan.cap;
-  a.direct = (int64_t)beams * plan.chunks > kPickLists;
+  // A prompt's CTA needs an SM to itself; where SMs are left over they help with the rare sums
+  // in 64 bits.
+  a.helpers = batch <= 16 ? kMaxHelpers : batch <= 32 ? 4 : batch <= 64 ? 2 : 1;
   a.gap = gap_of(vocab);
   a.stats = static_cast<ChunkStats *>(d_workspace);
   a.lists = reinterpret_cast<float2 *>(a.stats + rows * plan.chunks);

@@ -259,29 +259,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       : "memory");
 }
 
-// Packed and three-operand fp32 arithmetic.
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-  uint64_t r;
-  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-      "mov.b64 c, {%5, %6};\n\tfma.rn.f32x2 %0, a, b, c;\n\t}"
-      : "=l"(r)
-      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
-  return make_float2(__uint_as_float((uint32_t)r), __uint_as_float((uint32_t)(r >> 32)));
-}
-__device__ __forceinline__ float2 add2(float2 x, float2 y) {
-  uint64_t r;
-  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-      "add.rn.f32x2 %0, a, b;\n\t}"
-      : "=l"(r)
-      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
-  return make_float2(__uint_as_float((uint32_t)r), __uint_as_float((uint32_t)(r >> 32)));
-}
-
 template <typename T> struct Half;
 template <> struct Half<__nv_bfloat16> {
   static constexpr uint32_t kType = 1;
