@@ -29,10 +29,8 @@
 namespace tabby {
 namespace {
 
-constexpr int kScanThreads = 256;
+constexpr int kScanThreads = 128;
 constexpr int kScanWarps = kScanThreads / 32;
-constexpr int kPickThreads = 1024;
-constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kMaxHelpers = 8;
 constexpr int kPickCap = 1024;  // keys a prompt's selection may keep
 
@@ -182,7 +180,7 @@ __device__ __noinline__ int exact_list(const float *x, int n, int e0, int k, flo
 
 // NV pieces a thread: NV * kN logits in registers.
 template <typename T, int NV>
-__global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+__global__ void __launch_bounds__(kScanThreads, 6) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
   constexpr int kN = Vec16<T>::kN, kE = NV * kN;
   __shared__ float s_max[kScanWarps], s_sum[kScanWarps];
   __shared__ uint32_t s_bound[kScanWarps];
@@ -202,9 +200,9 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   const T *x0 = row_of<T>(a, row);
   const int lead = lead_of(x0);
   const T *base = x0 - lead;
-  const int pieces = (int)(((int64_t)lead + a.vocab + kN - 1) / kN);
-  const int v0 = (int)((int64_t)chunk * pieces / a.chunks);
-  const int v1 = (int)((int64_t)(chunk + 1) * pieces / a.chunks);
+  const int pieces = (lead + a.vocab + kN - 1) / kN;
+  const int even = pieces / a.chunks, more = pieces - even * a.chunks;
+  const int v0 = chunk * even + min(chunk, more), v1 = v0 + even + (chunk < more ? 1 : 0);
   float x[kE];
   if ((int64_t)v0 * kN >= lead && (int64_t)v1 * kN - lead <= a.vocab) {  // whole pieces only
     const T *p = base + (int64_t)(v0 + tid) * kN;
@@ -287,14 +285,16 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   }
   // Candidates: no smaller than the bound, above -inf.
   const float least = bound <= order_key(-INFINITY) ? -3.402823466e38f : key_value(bound);
-  auto element = [&](int j, int i) { return (v0 + j * kScanThreads + tid) * kN - lead + i; };
   if (top >= least) {
+    unsigned long long pass = 0;
 #pragma unroll
-    for (int i = 0; i < kE; i++)
-      if (x[i] >= least) {
-        const int at = atomicAdd(&s_count, 1);
-        if (at < a.cap) list[at] = make_float2(x[i], __int_as_float(element(i / kN, i % kN)));
-      }
+    for (int i = 0; i < kE; i++) pass |= x[i] >= least ? 1ull << i : 0ull;
+    int at = atomicAdd(&s_count, __popcll(pass));
+    for (; pass; pass &= pass - 1, at++) {
+      const int i = __ffsll(pass) - 1;
+      const int e = (v0 + i / kN * kScanThreads + tid) * kN - lead + i % kN;
+      if (at < a.cap) list[at] = make_float2(to_f32(x0[e]), __int_as_float(e));
+    }
   }
   __syncthreads();
   int count = s_count;
@@ -319,11 +319,17 @@ struct Cand {
   float x;
   int32_t beam, token;
 };
-// Within a beam the logits decide (their keys could round to the same), between beams the keys;
-// ties go to the lower beam, then token.
+// The larger key, then the lower beam; within a beam the larger logit (different ones can round
+// to the same key), then the lower token. (Within a beam keys rise with the logits.)
 __device__ __forceinline__ bool stands_before(const Cand &p, const Cand &q) {
-  if (p.beam == q.beam) return p.x > q.x || (p.x == q.x && p.token < q.token);
-  return p.key > q.key || (p.key == q.key && p.beam < q.beam);
+  if (p.key != q.key) return p.key > q.key;
+  if (p.beam != q.beam) return p.beam < q.beam;
+  return p.x > q.x || (p.x == q.x && p.token < q.token);
+}
+// Order-preserving integer of a key, -0 folded onto +0.
+__device__ __forceinline__ int64_t key_bits(double k) {
+  const int64_t b = __double_as_longlong(k + 0.0);
+  return b ^ (int64_t)((uint64_t)(b >> 63) >> 1);
 }
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -347,13 +353,65 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid_constant__ BeamArgs a) {
+// exp(d) for d <= 0 in 64 bits: 2^n 2^f with n the nearest integer to d log2(e) and 2^f by its
+// Taylor polynomial of degree 10 on [-1/2, 1/2] (off by less than 3e-13); 0 below 2^-1000.
+__device__ __forceinline__ double exp_below(double d) {
+  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+  const double t = d * 1.4426950408889634;
+  if (!(t > -1000.0)) return 0.0;
+  const double r = t + kRound, f = t - (r - kRound);
+  double p = 7.0549116208011209e-09;
+  p = fma(p, f, 1.0178086009239696e-07);
+  p = fma(p, f, 1.3215486790144305e-06);
+  p = fma(p, f, 1.5252733804059838e-05);
+  p = fma(p, f, 0.00015403530393381606);
+  p = fma(p, f, 0.0013333558146428441);
+  p = fma(p, f, 0.0096181291076284769);
+  p = fma(p, f, 0.055504108664821576);
+  p = fma(p, f, 0.24022650695910069);
+  p = fma(p, f, 0.69314718055994529);
+  p = fma(p, f, 1);
+  return __longlong_as_double(__double_as_longlong(p) + (__double_as_longlong(r) << 52));
+}
+// A CTA's share of sum exp(x - m) over the logits of row `row`, in 64 bits, to `to` (in the
+// cluster's first CTA).
+template <typename T, int kThreads>
+__device__ __noinline__ void share_sum(const BeamArgs &a, int row, float m, int helper,
+                                       double *s_warp, uint32_t to) {
+  constexpr int kWarps = kThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const T *x = row_of<T>(a, row);
+  const int n = (a.vocab + a.helpers - 1) / a.helpers, end = min(a.vocab, (helper + 1) * n);
+  double sum = 0;
+  for (int v = helper * n + tid; v < end; v += 8 * kThreads) {
+    float y[8];  // all on their way before the first is used
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      y[i] = v + i * kThreads < end ? to_f32(x[v + i * kThreads]) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum += exp_below((double)y[i] - (double)m);
+  }
+  sum = warp_sum(sum);
+  __syncthreads();
+  if (lane == 0) s_warp[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    sum = warp_sum(lane < kWarps ? s_warp[lane] : 0.0);
+    if (lane == 0) store_cluster(to, sum);
+  }
+}
+
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_constant__ BeamArgs a) {
+  constexpr int kWarps = kThreads / 32;
   __shared__ double s_lse[TABBY_BEAM_MAX], s_score[TABBY_BEAM_MAX];
-  __shared__ double s_bound[kPickWarps];
+  __shared__ double s_bound[kWarps];
+  __shared__ int s_sums[kWarps];
+  __shared__ int64_t s_key[kPickCap];
   __shared__ Cand s_cand[kPickCap];
   __shared__ int16_t s_order[kPickCap];
   __shared__ int s_rank[kPickCap];
+  int *s_end = s_rank;  // of the threads' lists, before anything is ranked
   __shared__ float s_rowmax[TABBY_BEAM_MAX];
   __shared__ uint8_t s_done[TABBY_BEAM_MAX];
   __shared__ uint32_t s_again[TABBY_BEAM_MAX], s_need;
@@ -363,37 +421,22 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
   const int row0 = b * a.beams, lists = a.beams * a.chunks;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const ChunkStats *stats = a.stats + (int64_t)row0 * a.chunks;
-  // This CTA's share of sum exp(x - m) over beam i's logits, in 64 bits.
-  auto share = [&](int i, float m, uint32_t to) {
-    const T *x = row_of<T>(a, row0 + i);
-    const int n = (a.vocab + a.helpers - 1) / a.helpers;
-    double sum = 0;
-    for (int v = helper * n + tid; v < min(a.vocab, (helper + 1) * n); v += kPickThreads)
-      sum += exp((double)to_f32(x[v]) - (double)m);
-    sum = warp_sum(sum);
-    __syncthreads();
-    if (lane == 0) s_bound[warp] = sum;
-    __syncthreads();
-    if (warp == 0) {
-      sum = warp_sum(s_bound[lane]);
-      if (lane == 0) store_cluster(to, sum);
-    }
-  };
   if (helper > 0) {  // waits for the first CTA's word
     cluster_arrive();
     cluster_wait();
     if (load_cluster(in_first_cta(&s_need)))
       for (int i = 0; i < a.beams; i++)
         if (load_cluster(in_first_cta(&s_again[i])))
-          share(i, __uint_as_float(load_cluster(in_first_cta(&s_rowmax[i]))),
-                in_first_cta(&s_part[helper][i]));
+          share_sum<T, kThreads>(a, row0 + i,
+                                 __uint_as_float(load_cluster(in_first_cta(&s_rowmax[i]))),
+                                 helper, s_bound, in_first_cta(&s_part[helper][i]));
     cluster_arrive();
     cluster_wait();
     return;
   }
   // Log-sum-exps, a warp a beam.
   bool bad = false;
-  for (int i = warp; i < a.beams; i += kPickWarps) {
+  for (int i = warp; i < a.beams; i += kWarps) {
     const float score = a.scores[row0 + i];
     const bool done = a.finished && a.finished[row0 + i] && score != -INFINITY;
     float m = -INFINITY;
@@ -429,7 +472,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
   };
   if (tid == 0) a.status[b] = bad ? TABBY_EINPUT : TABBY_OK;
   if (bad) {
-    for (int j = tid; j < a.n_out; j += kPickThreads) write(j, true, Cand());
+    for (int j = tid; j < a.n_out; j += kThreads) write(j, true, Cand());
     if (tid == 0) s_need = 0;
     cluster_arrive();
     cluster_wait();
@@ -460,12 +503,12 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
     c.key = s_score[i];
     return c;
   };
-  // A bound below the n_out-th largest of the threads' values (-inf where there are fewer), so
-  // that at least n_out keys are no smaller: by bisection over the values rounded down to fp32.
+  // A bound that at least n_out keys reach: the n_out-th largest of the threads' values (-inf
+  // where there are fewer), rounded down, by bisection over its upper 18 bits as fp32.
   auto bound_of = [&](double top) {
     const uint32_t key = order_key(__double2float_rd(top));
     uint32_t kth = 0;
-    for (int bit = 31; bit >= 0; bit--) {
+    for (int bit = 31; bit >= 14; bit--) {
       const uint32_t probe = kth | 1u << bit;
       if (__syncthreads_count(key >= probe) >= a.n_out) kth = probe;
     }
@@ -476,35 +519,60 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
     const int at = atomicAdd(&s_count, 1);
     if (at < kPickCap) s_cand[at] = c;
   };
-  // What is no smaller than a bound, less what more exact keys might bring up. Lists go round
-  // the warps, 32 at a time a warp, and only those whose best passes are read.
+  // Goes over the entries of the lists whose best reaches `least`: a thread looks at a list,
+  // their entries are laid end to end and then shared out evenly.
+  auto each_entry = [&](double least, auto use) {
+    for (int l0 = 0; l0 < lists; l0 += kThreads) {
+      const int l = l0 + tid;
+      int count = l < lists ? stats[l].count : 0;
+      if (count > 0 && !(list_top(l) >= least)) count = 0;
+      int end = count;  // inclusive over the threads
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += y;
+      }
+      __syncthreads();
+      if (lane == 31) s_sums[warp] = end;
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) {
+        if (w < warp) end += s_sums[w];
+        all += s_sums[w];
+      }
+      s_end[tid] = end;
+      __syncthreads();
+      for (int f = tid; f < all; f += kThreads) {
+        int lo = 0;  // the first list that ends behind f
+#pragma unroll
+        for (int o = kThreads / 2; o > 0; o >>= 1)
+          if (s_end[lo + o - 1] <= f) lo += o;
+        use(entry(l0 + lo, f - (lo > 0 ? s_end[lo - 1] : 0)));
+      }
+    }
+  };
+  // What is no smaller than a bound, less what more exact keys might bring up.
   auto collect = [&](double bound) {
     const double least = bound - 2 * a.gap;
     if (tid == 0) s_count = 0;
     __syncthreads();
-    for (int l0 = 0; l0 < lists; l0 += kPickThreads) {
-      const int l = l0 + lane * kPickWarps + warp;
-      const int count = l < lists ? stats[l].count : 0;
-      unsigned pass = __ballot_sync(0xffffffffu, count > 0 && list_top(l) >= least);
-      for (; pass; pass &= pass - 1) {
-        const int f = __ffs(pass) - 1, n = __shfl_sync(0xffffffffu, count, f);
-        for (int e = lane; e < n; e += 32) keep(entry(l0 + f * kPickWarps + warp, e), least);
-      }
-    }
-    for (int i = tid; i < a.beams; i += kPickThreads)
+    each_entry(least, [&](const Cand &c) { keep(c, least); });
+    for (int i = tid; i < a.beams; i += kThreads)
       if (s_done[i]) keep(finished(i), least);
     __syncthreads();
   };
   // A bound from the lists' bests; where too much passes it, one from the entries.
   double top = -INFINITY;
-  for (int l = tid; l < lists; l += kPickThreads) top = fmax(top, list_top(l));
-  collect(bound_of(top));
+  for (int l = lane * kWarps + warp; l < lists; l += kThreads) top = fmax(top, list_top(l));
+  double bound = bound_of(top);
+  collect(bound);
   if (s_count > kPickTight) {
     top = -INFINITY;
-    for (int u = warp; u < 4 * lists; u += kPickWarps)  // a quarter of a list
-      for (int e = (u & 3) * 32 + lane; e < stats[u >> 2].count; e += 128)
-        top = fmax(top, entry(u >> 2, e).key);
-    collect(bound_of(top));
+    each_entry(bound, [&](const Cand &c) { top = fmax(top, c.key); });
+    __syncthreads();
+    bound = fmax(bound, bound_of(top));
+    collect(bound);
   }
   // The lse of the marked beams in 64 bits, from all their logits, with the cluster's help.
   auto refine = [&]() {
@@ -512,10 +580,11 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
     cluster_arrive();
     cluster_wait();
     for (int i = 0; i < a.beams; i++)
-      if (s_again[i]) share(i, s_rowmax[i], in_first_cta(&s_part[0][i]));
+      if (s_again[i])
+        share_sum<T, kThreads>(a, row0 + i, s_rowmax[i], 0, s_bound, in_first_cta(&s_part[0][i]));
     cluster_arrive();
     cluster_wait();
-    for (int i = tid; i < a.beams; i += kPickThreads) {
+    for (int i = tid; i < a.beams; i += kThreads) {
       if (!s_again[i]) continue;
       double sum = 0;
       for (int k = 0; k < a.helpers; k++) sum += s_part[k][i];
@@ -528,11 +597,11 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
     // Too many for the table, by ties: with all keys exact, the best one after the other.
     __syncthreads();
     if (tid == 0) s_count = 0;
-    for (int i = tid; i < a.beams; i += kPickThreads)
+    for (int i = tid; i < a.beams; i += kThreads)
       s_again[i] = !s_done[i] && s_rowmax[i] > -INFINITY;
     __syncthreads();
     refine();
-    __shared__ Cand s_best[kPickWarps], s_last;
+    __shared__ Cand s_best[kWarps], s_last;
     Cand last;
     last.key = INFINITY;
     last.x = INFINITY;
@@ -546,9 +615,8 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
             (best.beam < 0 || stands_before(c, best)))
           best = c;
       };
-      for (int l = warp; l < lists; l += kPickWarps)
-        for (int e = lane; e < stats[l].count; e += 32) consider(entry(l, e));
-      for (int i = tid; i < a.beams; i += kPickThreads)
+      each_entry(-INFINITY, consider);
+      for (int i = tid; i < a.beams; i += kThreads)
         if (s_done[i]) consider(finished(i));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -563,7 +631,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
       __syncthreads();
       if (tid == 0) {
         best = s_best[0];
-        for (int w = 1; w < kPickWarps; w++)
+        for (int w = 1; w < kWarps; w++)
           if (s_best[w].beam >= 0 && (best.beam < 0 || stands_before(s_best[w], best)))
             best = s_best[w];
         s_last = best;
@@ -577,18 +645,24 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
   }
   const int n = s_count;
   auto rank = [&]() {  // s_order[j]: the candidate of rank j; a few threads a candidate
-    const int parts = max(1, kPickThreads / max(n, 1));
-    for (int i = tid; i < n; i += kPickThreads) s_rank[i] = 0;
+    const int parts = max(1, kThreads / max(n, 1));
+    for (int i = tid; i < n; i += kThreads) {
+      s_rank[i] = 0;
+      s_key[i] = key_bits(s_cand[i].key);
+    }
     __syncthreads();
-    for (int i = tid; i < n * parts; i += kPickThreads) {
+    for (int i = tid; i < n * parts; i += kThreads) {
       const int p = i / n, me = i - p * n;
-      const Cand c = s_cand[me];
+      const int64_t key = s_key[me];
       int r = 0;
-      for (int k = p; k < n; k += parts) r += stands_before(s_cand[k], c) ? 1 : 0;
+      for (int k = p; k < n; k += parts) {
+        const int64_t other = s_key[k];
+        if (other > key || (other == key && stands_before(s_cand[k], s_cand[me]))) r++;
+      }
       if (r) atomicAdd(&s_rank[me], r);
     }
     __syncthreads();
-    for (int i = tid; i < n; i += kPickThreads) s_order[s_rank[i]] = (int16_t)i;
+    for (int i = tid; i < n; i += kThreads) s_order[s_rank[i]] = (int16_t)i;
     __syncthreads();
   };
   rank();
@@ -596,7 +670,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
   // those that are as close to the last one chosen.
   bool close = false;
   const double lowest = n > 0 ? s_cand[s_order[min(n, a.n_out) - 1]].key - a.gap : 0.0;
-  for (int j = tid; !many && j < n - 1; j += kPickThreads) {
+  for (int j = tid; !many && j < n - 1; j += kThreads) {
     const Cand p = s_cand[s_order[j]], q = s_cand[s_order[j + 1]];
     if (q.key >= lowest && p.beam != q.beam && p.key - q.key < a.gap) {
       if (!s_done[p.beam]) s_again[p.beam] = 1, close = true;
@@ -606,7 +680,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
   const bool again = __syncthreads_or(close);
   if (again) {
     refine();
-    for (int i = tid; i < n; i += kPickThreads)
+    for (int i = tid; i < n; i += kThreads)
       if (const int k = s_cand[i].beam; s_again[k])
         s_cand[i].key = s_score[k] + ((double)s_cand[i].x - s_lse[k]);
     __syncthreads();
@@ -618,7 +692,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) beam_pick_kernel(const __grid
     cluster_wait();
     cluster_arrive();
   }
-  for (int j = tid; j < a.n_out; j += kPickThreads)
+  for (int j = tid; j < a.n_out; j += kThreads)
     write(j, j >= n, j < n ? s_cand[s_order[j]] : Cand());
   if (!again && !many) {
     __syncwarp();
@@ -639,7 +713,7 @@ ScanPlan scan_plan(int64_t rows, int32_t vocab, int32_t dtype, int32_t n_out) {
     return (int)((pieces + (int64_t)nv * kScanThreads - 1) / ((int64_t)nv * kScanThreads));
   };
   ScanPlan p;
-  p.nv = 32 / n;
+  p.nv = 48 / n;
   if (rows * chunks(p.nv) < 148) p.nv = 16 / n;  // few rows: half the chunk, twice the CTAs
   p.chunks = chunks(p.nv);
   p.cap = std::max(128, 4 * n_out);
@@ -651,12 +725,14 @@ cudaError_t launch_beam(const BeamArgs &a, int nv, cudaStream_t q) {
   constexpr int kN = Vec16<T>::kN;
   const dim3 grid((unsigned)a.batch * (unsigned)a.beams * (unsigned)a.chunks);
   cudaError_t err =
-      nv == 32 / kN ? launch_pdl(beam_scan_kernel<T, 32 / kN>, grid, kScanThreads, 0, q, a)
+      nv == 48 / kN ? launch_pdl(beam_scan_kernel<T, 48 / kN>, grid, kScanThreads, 0, q, a)
                     : launch_pdl(beam_scan_kernel<T, 16 / kN>, grid, kScanThreads, 0, q, a);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.batch * a.helpers));
-  cfg.blockDim = dim3(kPickThreads);
+  // Many lists with many entries: more threads.
+  const int threads = a.beams * a.n_out > 512 ? 1024 : 256;
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = q;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -665,7 +741,8 @@ cudaError_t launch_beam(const BeamArgs &a, int nv, cudaStream_t q) {
   attr[1].val.clusterDim = {(unsigned)a.helpers, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, beam_pick_kernel<T>, a);
+  return threads == 256 ? cudaLaunchKernelEx(&cfg, beam_pick_kernel<T, 256>, a)
+                        : cudaLaunchKernelEx(&cfg, beam_pick_kernel<T, 1024>, a);
 }
 
 int check_sizes(int32_t batch, int32_t beams, int32_t vocab, int32_t n_out) {
@@ -757,9 +834,8 @@ int tabby_beam_step_async(int32_t device, const void *d_logits, int32_t dtype,
   const ScanPlan plan = scan_plan((int64_t)rows, vocab, dtype, n_out);
   a.chunks = plan.chunks;
   a.cap = plan.cap;
-  // A prompt's CTA needs an SM to itself; where SMs are left over they help with the rare sums
-  // in 64 bits.
-  a.helpers = batch <= 16 ? kMaxHelpers : batch <= 32 ? 4 : batch <= 64 ? 2 : 1;
+  // Where SMs are left over they help a prompt's CTA with the rare sums in 64 bits.
+  a.helpers = batch <= 64 ? kMaxHelpers : batch <= 256 ? 2 : 1;
   a.gap = gap_of(vocab);
   a.stats = static_cast<ChunkStats *>(d_workspace);
   a.lists = reinterpret_cast<float2 *>(a.stats + rows * plan.chunks);
