@@ -104,6 +104,7 @@ TABBY_TREE_MAX_NODES = 64
 TABBY_TREE_MAX_DIM = 128
 TABBY_F32, TABBY_BF16, TABBY_F16 = 0, 1, 2
 DECODE_LIB_PATH = os.path.join(_PKG, "lib", "libtabbydecode.so")
+DECODE_TORCH_PATH = os.path.join(_PKG, "lib", "tabby_decode_torch.so")
 
 
 class StateLayout(ctypes.Structure):

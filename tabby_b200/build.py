@@ -1,11 +1,12 @@
 """Build the shared libraries in-tree with nvcc for sm_100a.
 
-    python -m tabby_b200.build        # -> tabby_b200/lib/libtabby{sample,decode}.so
+    python -m tabby_b200.build        # -> tabby_b200/lib/
 
 libtabbysample.so (include/tabby_sample.h) is the sampler, libtabbydecode.so
 (include/tabby_decode.h) the decode operators for several hypotheses a sequence. Both are
 plain C-ABI shared objects that do not link against torch. CUDA's runtime is linked
-statically so they only need the driver.
+statically so they only need the driver. tabby_decode_torch.so is the Python side of the
+second on torch tensors (decode.py), an extension module built with g++ against torch.
 """
 from __future__ import annotations
 
@@ -24,6 +25,7 @@ SOURCES = ["sampler_kernels.cu", "capi.cu", "noalloc.cu", "softmax_rows.cu", "lm
            "exchange.cu"]
 DECODE_LIB = os.path.join(LIBDIR, "libtabbydecode.so")
 DECODE_SOURCES = ["decode_capi.cu", "beam.cu", "states.cu", "tree_attention.cu"]
+DECODE_TORCH = os.path.join(LIBDIR, "tabby_decode_torch.so")
 HEADERS = ["decode_internal.h", "finalize.cuh", "js_math.cuh", "sampler_internal.h", "sm100.cuh",
            "warp_sort.cuh"]
 
@@ -77,9 +79,29 @@ def _build_lib(lib_path: str, sources: list, verbose: bool, defines: tuple) -> N
         os.remove(o)
 
 
+def _build_torch() -> None:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    libs = cpp_extension.library_paths()
+    includes = [os.path.join(ROOT, "include"), "/usr/local/cuda/include",
+                sysconfig.get_paths()["include"], *cpp_extension.include_paths()]
+    tmp = DECODE_TORCH + ".tmp"
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+          "-DTORCH_EXTENSION_NAME=tabby_decode_torch",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *[f"-I{i}" for i in includes], os.path.join(CSRC, "decode_torch.cpp"), "-o", tmp,
+          f"-L{LIBDIR}", "-l:libtabbydecode.so", *[f"-L{p}" for p in libs], "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
+          "-lc10", "-lc10_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"],
+         "g++ failed for decode_torch.cpp")
+    os.replace(tmp, DECODE_TORCH)
+
+
 def build(force: bool = False, verbose: bool = False, out: str | None = None,
           defines: tuple = ()) -> str:
-    """Compile both libraries in-tree and return the sampler's path; with `out`, only
+    """Compile the libraries in-tree and return the sampler's path; with `out`, only
     SOURCES into that path. `defines` adds -D flags (e.g. TABBY_CHECKS=1 for the
     self-checking debug build)."""
     if out is not None:
@@ -88,6 +110,8 @@ def build(force: bool = False, verbose: bool = False, out: str | None = None,
     for lib_path, sources in ((LIB, SOURCES), (DECODE_LIB, DECODE_SOURCES)):
         if force or _stale(lib_path, sources):
             _build_lib(lib_path, sources, verbose, defines)
+    if force or _stale(DECODE_TORCH, ["decode_torch.cpp"]):
+        _build_torch()
     return LIB
 
 
