@@ -5,7 +5,10 @@
 // what it overwrites is read by nobody else and no second buffer is needed. It first loads all
 // rows that move, then stores them. W is the widest power of two that divides the layout (and,
 // for many beams, keeps one value a beam in registers).
+#include <math.h>
+
 #include <algorithm>
+#include <cmath>
 
 #include "decode_internal.h"
 
@@ -23,8 +26,9 @@ struct ReorderArgs {
   tabby_state_layout l;
   int32_t beams;
   const int32_t *parents, *lengths;
-  int32_t vpe;        // columns an entry
-  int64_t chunks;     // blocks a segment
+  int32_t vpe;     // columns an entry
+  int32_t packed;  // a segment's entries lie end to end
+  int64_t chunks;  // blocks a segment
 };
 
 template <int W> struct Vec;
@@ -34,9 +38,12 @@ template <> struct Vec<4> { typedef uint32_t T; };
 template <> struct Vec<2> { typedef uint16_t T; };
 template <> struct Vec<1> { typedef uint8_t T; };
 
-// blockIdx.x = ((state * batch + b) * segments + g) * chunks + chunk.
-template <int W, int K>
-__global__ void __launch_bounds__(kMoveThreads) reorder_kernel(ReorderArgs a, StatePtrs s,
+// blockIdx.x = ((state * batch + b) * segments + g) * chunks + chunk. A thread takes U columns of
+// a chunk, so that a row's part of it is U * 128 * W contiguous bytes and enough loads are on
+// their way before the first store.
+template <int W, int K, int U>
+__global__ void __launch_bounds__(kMoveThreads) reorder_kernel(const __grid_constant__ ReorderArgs a,
+                                                               const __grid_constant__ StatePtrs s,
                                                                int32_t batch) {
   typedef typename Vec<W>::T V;
   __shared__ int32_t from[K];
@@ -58,20 +65,34 @@ __global__ void __launch_bounds__(kMoveThreads) reorder_kernel(ReorderArgs a, St
   const int64_t len =
       a.lengths ? min(max(a.lengths[b], 0), a.l.entries) : a.l.entries;
   __syncthreads();
-  const int64_t base = chunk * kMoveThreads;  // the block's first column of the segment
-  const uint32_t local = (uint32_t)(base % a.vpe) + threadIdx.x;
-  const int64_t t = base / a.vpe + local / (uint32_t)a.vpe;
-  if (t >= len) return;
-  unsigned char *p = s.p[state] + (int64_t)b * a.beams * a.l.row_stride +
-                     g * a.l.segment_stride + t * a.l.entry_stride +
-                     (int64_t)(local % (uint32_t)a.vpe) * W;
-  V v[K];
+  const int64_t base = chunk * (U * kMoveThreads);  // the block's first column of the segment
+  const int64_t cols = len * a.vpe;
+  if (base >= cols) return;
+  unsigned char *p0 = s.p[state] + (int64_t)b * a.beams * a.l.row_stride + g * a.l.segment_stride;
+  V v[U][K];
+  unsigned char *p[U];
 #pragma unroll
-  for (int i = 0; i < K; i++)
-    if (from[i] >= 0) v[i] = *reinterpret_cast<const V *>(p + from[i] * a.l.row_stride);
+  for (int j = 0; j < U; j++) {
+    const uint32_t i = j * kMoveThreads + threadIdx.x;
+    p[j] = nullptr;
+    if (base + i < cols) {
+      if (a.packed) {
+        p[j] = p0 + (base + i) * W;
+      } else {
+        const uint32_t local = (uint32_t)(base % a.vpe) + i;
+        p[j] = p0 + (base / a.vpe + local / (uint32_t)a.vpe) * a.l.entry_stride +
+               (int64_t)(local % (uint32_t)a.vpe) * W;
+      }
+    }
 #pragma unroll
-  for (int i = 0; i < K; i++)
-    if (from[i] >= 0) *reinterpret_cast<V *>(p + i * a.l.row_stride) = v[i];
+    for (int k = 0; k < K; k++)
+      if (p[j] && from[k] >= 0) v[j][k] = *reinterpret_cast<const V *>(p[j] + from[k] * a.l.row_stride);
+  }
+#pragma unroll
+  for (int j = 0; j < U; j++)
+#pragma unroll
+    for (int k = 0; k < K; k++)
+      if (p[j] && from[k] >= 0) *reinterpret_cast<V *>(p[j] + k * a.l.row_stride) = v[j][k];
 }
 
 struct AcceptArgs {
@@ -93,7 +114,8 @@ struct AcceptArgs {
 // blockIdx.x = (cache * batch + b) * chunks + chunk. Every block walks its sequence's tree
 // (a few dozen steps over shared memory); the first block of a sequence writes the outcome.
 template <int W>
-__global__ void __launch_bounds__(kMoveThreads) accept_kernel(AcceptArgs a, StatePtrs s) {
+__global__ void __launch_bounds__(kMoveThreads) accept_kernel(const __grid_constant__ AcceptArgs a,
+                                                              const __grid_constant__ StatePtrs s) {
   typedef typename Vec<W>::T V;
   __shared__ int32_t parents[TABBY_TREE_MAX_NODES], tokens[TABBY_TREE_MAX_NODES];
   __shared__ int32_t sampled[TABBY_TREE_MAX_NODES], path[TABBY_TREE_MAX_NODES];
@@ -159,22 +181,40 @@ int vector_bytes(const tabby_state_layout &l, void *const *states, int32_t n, in
   return w;
 }
 
+// The same places as a layout with as few segments and as long entries as it allows.
+tabby_state_layout merged(tabby_state_layout l) {
+  if (l.segments > 1 && l.segment_stride == l.entry_bytes &&
+      l.entry_bytes * l.segments < (int64_t)1 << 31 &&
+      (l.entries == 1 || l.entry_stride >= l.entry_bytes * l.segments)) {  // [tokens][heads][dim]
+    l.entry_bytes *= l.segments;
+    l.segments = 1;
+  }
+  return l;
+}
+
+// Columns a thread, by the values it holds for each.
+constexpr int columns_of(int w, int k) {
+  return w * k <= 64 ? 4 : w * k <= 128 ? 2 : 1;
+}
+
 template <int W, int K>
-void reorder_launch(const ReorderArgs &a, const StatePtrs &s, int32_t batch, unsigned grid,
-                    cudaStream_t q) {
-  reorder_kernel<W, K><<<grid, kMoveThreads, 0, q>>>(a, s, batch);
+void reorder_launch(ReorderArgs a, const StatePtrs &s, int32_t n, int32_t batch, cudaStream_t q) {
+  constexpr int kColumns = columns_of(W, K) * kMoveThreads;
+  a.chunks = ((int64_t)a.l.entries * a.vpe + kColumns - 1) / kColumns;
+  const unsigned grid = (unsigned)((int64_t)n * batch * a.l.segments * a.chunks);
+  reorder_kernel<W, K, columns_of(W, K)><<<grid, kMoveThreads, 0, q>>>(a, s, batch);
 }
 
 template <int W>
-void reorder_launch_beams(const ReorderArgs &a, const StatePtrs &s, int32_t batch, unsigned grid,
+void reorder_launch_beams(const ReorderArgs &a, const StatePtrs &s, int32_t n, int32_t batch,
                           cudaStream_t q) {
-  if (a.beams <= 4) return reorder_launch<W, 4>(a, s, batch, grid, q);
-  if (a.beams <= 8) return reorder_launch<W, 8>(a, s, batch, grid, q);
-  if (a.beams <= 16) return reorder_launch<W, 16>(a, s, batch, grid, q);
+  if (a.beams <= 4) return reorder_launch<W, 4>(a, s, n, batch, q);
+  if (a.beams <= 8) return reorder_launch<W, 8>(a, s, n, batch, q);
+  if (a.beams <= 16) return reorder_launch<W, 16>(a, s, n, batch, q);
   if constexpr (W <= 8) {
-    if (a.beams <= 32) return reorder_launch<W, 32>(a, s, batch, grid, q);
+    if (a.beams <= 32) return reorder_launch<W, 32>(a, s, n, batch, q);
   }
-  if constexpr (W <= 4) reorder_launch<W, 64>(a, s, batch, grid, q);
+  if constexpr (W <= 4) reorder_launch<W, 64>(a, s, n, batch, q);
 }
 
 }  // namespace
@@ -199,15 +239,16 @@ int tabby_states_reorder_async(int32_t device, void *const *h_states, int32_t n_
     return decode_fail(TABBY_EINVAL, "states_reorder: states and parents must not be NULL");
   for (int32_t i = 0; i < n_states; i++)
     if (!h_states[i]) return decode_fail(TABBY_EINVAL, "states_reorder: state %d is NULL", i);
-  const int w = vector_bytes(*layout, h_states, n_states, beams <= 16 ? 16 : beams <= 32 ? 8 : 4);
   ReorderArgs a;
-  a.l = *layout;
+  a.l = merged(*layout);
+  const int w = vector_bytes(a.l, h_states, n_states, beams <= 16 ? 16 : beams <= 32 ? 8 : 4);
   a.beams = beams;
   a.parents = d_parents;
   a.lengths = d_lengths;
-  a.vpe = (int32_t)(layout->entry_bytes / w);
-  a.chunks = ((int64_t)layout->entries * a.vpe + kMoveThreads - 1) / kMoveThreads;
-  const double blocks = (double)batch * layout->segments * (double)a.chunks;
+  a.vpe = (int32_t)(a.l.entry_bytes / w);
+  a.packed = a.l.entries == 1 || a.l.entry_stride == a.l.entry_bytes;
+  const double blocks = (double)batch * a.l.segments *
+                        std::ceil((double)a.l.entries * a.vpe / kMoveThreads);
   if (blocks > 2147483647.0)
     return decode_fail(TABBY_EINVAL, "states_reorder: a state is too large for one launch");
   const int32_t most =
@@ -219,13 +260,12 @@ int tabby_states_reorder_async(int32_t device, void *const *h_states, int32_t n_
     const int32_t n = std::min(n_states - s0, most);
     StatePtrs s;
     for (int32_t i = 0; i < n; i++) s.p[i] = static_cast<unsigned char *>(h_states[s0 + i]);
-    const unsigned grid = (unsigned)((int64_t)n * batch * layout->segments * a.chunks);
     switch (w) {
-      case 16: reorder_launch_beams<16>(a, s, batch, grid, q); break;
-      case 8: reorder_launch_beams<8>(a, s, batch, grid, q); break;
-      case 4: reorder_launch_beams<4>(a, s, batch, grid, q); break;
-      case 2: reorder_launch_beams<2>(a, s, batch, grid, q); break;
-      default: reorder_launch_beams<1>(a, s, batch, grid, q); break;
+      case 16: reorder_launch_beams<16>(a, s, n, batch, q); break;
+      case 8: reorder_launch_beams<8>(a, s, n, batch, q); break;
+      case 4: reorder_launch_beams<4>(a, s, n, batch, q); break;
+      case 2: reorder_launch_beams<2>(a, s, n, batch, q); break;
+      default: reorder_launch_beams<1>(a, s, n, batch, q); break;
     }
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return decode_cuda_fail(err, "reorder_kernel launch");
@@ -277,11 +317,11 @@ int tabby_tree_accept_async(int32_t device, const int32_t *d_sampled,
   a.chunks = 1;
   int w = 1;
   if (n_caches > 0) {
-    w = vector_bytes(*layout, h_caches, n_caches, 16);
-    a.l = *layout;
-    a.entries = layout->entries;
-    a.vpe = (int32_t)(layout->entry_bytes / w);
-    a.chunks = ((int64_t)layout->segments * a.vpe + kMoveThreads - 1) / kMoveThreads;
+    a.l = merged(*layout);
+    w = vector_bytes(a.l, h_caches, n_caches, 16);
+    a.entries = a.l.entries;
+    a.vpe = (int32_t)(a.l.entry_bytes / w);
+    a.chunks = ((int64_t)a.l.segments * a.vpe + kMoveThreads - 1) / kMoveThreads;
   }
   const double blocks = (double)batch * (double)a.chunks;
   if (blocks > 2147483647.0)
