@@ -112,14 +112,13 @@ struct AcceptArgs {
 };
 
 // blockIdx.x = (cache * batch + b) * chunks + chunk. Every block walks its sequence's tree
-// (a few dozen steps over shared memory); the first block of a sequence writes the outcome.
+// (a warp finds each step's slot by a ballot); the first block of a sequence writes the outcome.
 template <int W>
 __global__ void __launch_bounds__(kMoveThreads) accept_kernel(const __grid_constant__ AcceptArgs a,
                                                               const __grid_constant__ StatePtrs s) {
   typedef typename Vec<W>::T V;
   __shared__ int32_t parents[TABBY_TREE_MAX_NODES], tokens[TABBY_TREE_MAX_NODES];
   __shared__ int32_t sampled[TABBY_TREE_MAX_NODES], path[TABBY_TREE_MAX_NODES];
-  __shared__ unsigned char used[TABBY_TREE_MAX_NODES];
   __shared__ int32_t n_path;
   int64_t u = blockIdx.x;
   const int64_t chunk = u % a.chunks;
@@ -134,19 +133,28 @@ __global__ void __launch_bounds__(kMoveThreads) accept_kernel(const __grid_const
     sampled[t] = a.sampled[b * a.sampled_batch_stride + t * a.sampled_stride];
   }
   __syncthreads();
-  if (t < a.nodes) used[t] = start >= 0 && start + t < a.entries && tree_sees(parents, t) != 0;
-  __syncthreads();
-  if (t == 0) {
-    int n = 0, cur = 0;
-    if (used[0] && parents[0] == -1) {
-      path[n++] = 0;
-      for (int j = 1; j < a.nodes; j++)  // a child stands behind its parent
-        if (used[j] && parents[j] == cur && tokens[j] == sampled[cur]) {
-          path[n++] = j;
-          cur = j;
-        }
+  if (t < 32) {  // a warp, two slots a lane
+    bool used[2];
+    for (int h = 0; h < 2; h++) {
+      const int j = t + 32 * h;
+      used[h] = j < a.nodes && start >= 0 && start + j < a.entries && tree_sees(parents, j) != 0;
     }
-    n_path = n;
+    int n = 0, cur = 0;
+    if (__shfl_sync(0xffffffffu, used[0], 0) && parents[0] == -1) {
+      while (true) {
+        if (t == 0) path[n] = cur;
+        n++;
+        const int want = sampled[cur];
+        const unsigned lo =
+            __ballot_sync(0xffffffffu, used[0] && parents[t] == cur && tokens[t] == want);
+        const unsigned hi = __ballot_sync(
+            0xffffffffu, used[1] && parents[t + 32] == cur && tokens[t + 32] == want);
+        if (lo) cur = __ffs(lo) - 1;
+        else if (hi) cur = 31 + __ffs(hi);
+        else break;
+      }
+    }
+    if (t == 0) n_path = n;
   }
   __syncthreads();
   const int n = n_path;
@@ -163,11 +171,19 @@ __global__ void __launch_bounds__(kMoveThreads) accept_kernel(const __grid_const
   if (col >= (int64_t)a.l.segments * a.vpe) return;
   unsigned char *p = s.p[cache] + b * a.l.row_stride + (col / a.vpe) * a.l.segment_stride +
                      start * a.l.entry_stride + (col % a.vpe) * W;
-  // path[r] >= r and the path rises, so no entry is overwritten before it is read.
-  for (int r = 1; r < n; r++)
-    if (path[r] != r)
-      *reinterpret_cast<V *>(p + r * a.l.entry_stride) =
-          *reinterpret_cast<const V *>(p + path[r] * a.l.entry_stride);
+  // path[r] >= r and the path rises, so no entry is overwritten before it is read; eight loads
+  // are on their way at a time.
+  for (int r0 = 1; r0 < n; r0 += 8) {
+    V v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (r0 + i < n && path[r0 + i] != r0 + i)
+        v[i] = *reinterpret_cast<const V *>(p + path[r0 + i] * a.l.entry_stride);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (r0 + i < n && path[r0 + i] != r0 + i)
+        *reinterpret_cast<V *>(p + (r0 + i) * a.l.entry_stride) = v[i];
+  }
 }
 
 // The widest power of two up to `most` that divides every address of the states.
