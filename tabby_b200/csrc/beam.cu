@@ -326,11 +326,34 @@ __device__ __forceinline__ bool stands_before(const Cand &p, const Cand &q) {
   if (p.beam != q.beam) return p.beam < q.beam;
   return p.x > q.x || (p.x == q.x && p.token < q.token);
 }
-// Order-preserving integer of a key, -0 folded onto +0.
+// Order-preserving integer of a key (-0 folded onto +0), and back.
 __device__ __forceinline__ int64_t key_bits(double k) {
   const int64_t b = __double_as_longlong(k + 0.0);
   return b ^ (int64_t)((uint64_t)(b >> 63) >> 1);
 }
+__device__ __forceinline__ double bits_key(int64_t b) {
+  return __longlong_as_double(b ^ (int64_t)((uint64_t)(b >> 63) >> 1));
+}
+// A prompt's candidates in shared memory, as integers that order them: the larger key, then the
+// smaller tie (beam, then falling logit), then the lower token.
+struct CandTable {
+  int64_t key[kPickCap];
+  uint64_t tie[kPickCap];
+  int32_t token[kPickCap];
+  __device__ __forceinline__ void put(int i, const Cand &c) {
+    key[i] = key_bits(c.key);
+    tie[i] = (uint64_t)c.beam << 32 | (uint32_t)~order_key(c.x);
+    token[i] = c.token;
+  }
+  __device__ __forceinline__ Cand get(int i) const {
+    Cand c;
+    c.key = bits_key(key[i]);
+    c.x = key_value(~(uint32_t)tie[i]);
+    c.beam = (int32_t)(tie[i] >> 32);
+    c.token = token[i];
+    return c;
+  }
+};
 
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -407,8 +430,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   __shared__ double s_lse[TABBY_BEAM_MAX], s_score[TABBY_BEAM_MAX];
   __shared__ double s_bound[kWarps];
   __shared__ int s_sums[kWarps];
-  __shared__ int64_t s_key[kPickCap];
-  __shared__ Cand s_cand[kPickCap];
+  __shared__ CandTable s_cand;
   __shared__ int16_t s_order[kPickCap];
   __shared__ int s_rank[kPickCap];
   int *s_end = s_rank;  // of the threads' lists, before anything is ranked
@@ -517,7 +539,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   auto keep = [&](const Cand &c, double least) {
     if (c.key < least) return;
     const int at = atomicAdd(&s_count, 1);
-    if (at < kPickCap) s_cand[at] = c;
+    if (at < kPickCap) s_cand.put(at, c);
   };
   // Goes over the entries of the lists whose best reaches `least`: a thread looks at a list,
   // their entries are laid end to end and then shared out evenly.
@@ -635,7 +657,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
           if (s_best[w].beam >= 0 && (best.beam < 0 || stands_before(s_best[w], best)))
             best = s_best[w];
         s_last = best;
-        if (best.beam >= 0) s_cand[s_count++] = best;
+        if (best.beam >= 0) s_cand.put(s_count++, best);
       }
       __syncthreads();
       last = s_last;
@@ -646,18 +668,17 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   const int n = s_count;
   auto rank = [&]() {  // s_order[j]: the candidate of rank j; a few threads a candidate
     const int parts = max(1, kThreads / max(n, 1));
-    for (int i = tid; i < n; i += kThreads) {
-      s_rank[i] = 0;
-      s_key[i] = key_bits(s_cand[i].key);
-    }
+    for (int i = tid; i < n; i += kThreads) s_rank[i] = 0;
     __syncthreads();
     for (int i = tid; i < n * parts; i += kThreads) {
       const int p = i / n, me = i - p * n;
-      const int64_t key = s_key[me];
+      const int64_t key = s_cand.key[me];
+      const uint64_t tie = s_cand.tie[me];
+      const int32_t token = s_cand.token[me];
       int r = 0;
       for (int k = p; k < n; k += parts) {
-        const int64_t other = s_key[k];
-        if (other > key || (other == key && stands_before(s_cand[k], s_cand[me]))) r++;
+        const bool less = s_cand.tie[k] < tie || (s_cand.tie[k] == tie && s_cand.token[k] < token);
+        r += s_cand.key[k] > key || (s_cand.key[k] == key && less) ? 1 : 0;
       }
       if (r) atomicAdd(&s_rank[me], r);
     }
@@ -669,9 +690,9 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   // Neighbours of different beams that are too close to be told apart by fp32 sums, down to
   // those that are as close to the last one chosen.
   bool close = false;
-  const double lowest = n > 0 ? s_cand[s_order[min(n, a.n_out) - 1]].key - a.gap : 0.0;
+  const double lowest = n > 0 ? s_cand.get(s_order[min(n, a.n_out) - 1]).key - a.gap : 0.0;
   for (int j = tid; !many && j < n - 1; j += kThreads) {
-    const Cand p = s_cand[s_order[j]], q = s_cand[s_order[j + 1]];
+    const Cand p = s_cand.get(s_order[j]), q = s_cand.get(s_order[j + 1]);
     if (q.key >= lowest && p.beam != q.beam && p.key - q.key < a.gap) {
       if (!s_done[p.beam]) s_again[p.beam] = 1, close = true;
       if (!s_done[q.beam]) s_again[q.beam] = 1, close = true;
@@ -681,8 +702,8 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   if (again) {
     refine();
     for (int i = tid; i < n; i += kThreads)
-      if (const int k = s_cand[i].beam; s_again[k])
-        s_cand[i].key = s_score[k] + ((double)s_cand[i].x - s_lse[k]);
+      if (const Cand c = s_cand.get(i); s_again[c.beam])
+        s_cand.key[i] = key_bits(s_score[c.beam] + ((double)c.x - s_lse[c.beam]));
     __syncthreads();
     rank();
   }
@@ -693,7 +714,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     cluster_arrive();
   }
   for (int j = tid; j < a.n_out; j += kThreads)
-    write(j, j >= n, j < n ? s_cand[s_order[j]] : Cand());
+    write(j, j >= n, j < n ? s_cand.get(s_order[j]) : Cand());
   if (!again && !many) {
     __syncwarp();
     cluster_wait();  // the others have read the word
