@@ -3,11 +3,11 @@
 //
 //   lse(i) = max + log(sum exp(x - max)),  key(i, v) = score(i) + (x - lse(i)) in 64 bits
 //
-//   beam_scan_kernel  reads every logit once. A CTA of 256 threads takes a chunk of a row (8192
-//                     logits, or 4096 where there are few rows) into registers, all loads at
+//   beam_scan_kernel  reads every logit once. A CTA of 128 threads takes a chunk of a row (6144
+//                     logits, or 2048 where there are few rows) into registers, all loads at
 //                     once; the chunk's maximum, its sum of exponentials and the logits that
 //                     can be among its n_out best are found from there. A bound on the n_out-th
-//                     best: of the 8 warps' thread maxima the ceil(n_out / 8) best each are at
+//                     best: of the 4 warps' thread maxima the ceil(n_out / 4) best each are at
 //                     least n_out logits, so all that matters is no smaller than the least of
 //                     them. Where more logits than a list holds pass it (ties, or warps without
 //                     logits) the exact n_out-th best is found by bisection over the values.
@@ -60,12 +60,12 @@ struct BeamArgs {
   float2 *lists;      // [rows][chunks][cap]: logit, token (bits)
 };
 
-// A row's terms exp(x - max) are each off by at most (3 |x - max| + 4) u relative (u = 2^-24:
+// A row's terms exp(x - max) are each off by at most (2.25 |x - max| + 4) u relative (u = 2^-24:
 // the difference, its product with log2(e), the constant; ex2's 4 u); weighted by the
-// probabilities |x - max| averages to at most ln(vocab). Their fp32 sums add 14 u (runs of 8, 2,
-// a warp's tree). Two lse's differ by twice that.
+// probabilities |x - max| averages to at most ln(vocab). Their fp32 sums add 13 u (runs of 6, 3
+// sums of those, 5 steps of a warp's tree). Two lse's differ by twice that.
 double gap_of(int32_t vocab) {
-  return 2.0 * (3.0 * log((double)std::max(vocab, 2)) + 20.0) * 5.9604644775390625e-8;
+  return 2.0 * (2.25 * log((double)std::max(vocab, 2)) + 17.0) * 5.9604644775390625e-8;
 }
 
 template <typename T> struct Vec16;  // the values of 16 bytes
@@ -180,7 +180,7 @@ __device__ __noinline__ int exact_list(const float *x, int n, int e0, int k, flo
 
 // NV pieces a thread: NV * kN logits in registers.
 template <typename T, int NV>
-__global__ void __launch_bounds__(kScanThreads, 6) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+__global__ void __launch_bounds__(kScanThreads, 7) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
   constexpr int kN = Vec16<T>::kN, kE = NV * kN;
   __shared__ float s_max[kScanWarps], s_sum[kScanWarps];
   __shared__ uint32_t s_bound[kScanWarps];
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kScanThreads, 6) beam_scan_kernel(const __grid
       max3_nan(max3_nan(mx[0], mx[1], x[kE - 4]), max3_nan(mx[2], mx[3], x[kE - 3]),
                max3_nan(x[kE - 2], x[kE - 1], x[0]));
   const bool bad = !(top < INFINITY);
-  // The warp's maximum and its ceil(n_out / 8)-th best thread maximum.
+  // The warp's maximum and its ceil(n_out / 4)-th best thread maximum.
   const uint32_t key = bad ? 0u : order_key(top);
   uint32_t rest = key, kth = 0;
   const uint32_t best = __reduce_max_sync(0xffffffffu, key);
@@ -248,17 +248,18 @@ __global__ void __launch_bounds__(kScanThreads, 6) beam_scan_kernel(const __grid
   }
   const float wmax = best ? key_value(best) : -INFINITY;
   // The sum relative to the warp's maximum.
-  float2 sum[2] = {};
+  float2 sum[4] = {};
   if (wmax > -INFINITY) {
     constexpr float kLog2e = 1.4426950408889634f;
     const float2 m2 = make_float2(-wmax, -wmax), l2 = make_float2(kLog2e, kLog2e);
 #pragma unroll
     for (int i = 0; i < kE; i += 2) {
       const float2 t = mul2(add2(make_float2(x[i], x[i + 1]), m2), l2);
-      sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], make_float2(ex2_fast(t.x), ex2_fast(t.y)));
+      sum[(i >> 1) & 3] = add2(sum[(i >> 1) & 3], make_float2(ex2_fast(t.x), ex2_fast(t.y)));
     }
   }
-  float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+  const float2 sums = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+  float total = sums.x + sums.y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) {
@@ -406,13 +407,13 @@ __device__ __noinline__ void share_sum(const BeamArgs &a, int row, float m, int 
   const T *x = row_of<T>(a, row);
   const int n = (a.vocab + a.helpers - 1) / a.helpers, end = min(a.vocab, (helper + 1) * n);
   double sum = 0;
-  for (int v = helper * n + tid; v < end; v += 8 * kThreads) {
-    float y[8];  // all on their way before the first is used
+  for (int v = helper * n + tid; v < end; v += 16 * kThreads) {
+    float y[16];  // all on their way before the first is used
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+    for (int i = 0; i < 16; i++)
       y[i] = v + i * kThreads < end ? to_f32(x[v + i * kThreads]) : -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 8; i++) sum += exp_below((double)y[i] - (double)m);
+    for (int i = 0; i < 16; i++) sum += exp_below((double)y[i] - (double)m);
   }
   sum = warp_sum(sum);
   __syncthreads();
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   }
 }
 
-// Chunks of a row: at most 256 threads' worth of pieces each.
+// Chunks of a row: at most 128 threads' worth of pieces each.
 struct ScanPlan {
   int nv;      // pieces a thread
   int chunks;  // a row
@@ -735,7 +736,9 @@ ScanPlan scan_plan(int64_t rows, int32_t vocab, int32_t dtype, int32_t n_out) {
   };
   ScanPlan p;
   p.nv = 48 / n;
-  if (rows * chunks(p.nv) < 148) p.nv = 16 / n;  // few rows: half the chunk, twice the CTAs
+  // Few rows: smaller chunks, so that every SM has some (4 rows of 151936: 152 chunks of 6144 leave
+  // no SM two; as 300 of 2048 the scan takes 6.0 us, as 100 it took 7.2).
+  if (rows * chunks(p.nv) < 148) p.nv = 16 / n;
   p.chunks = chunks(p.nv);
   p.cap = std::max(128, 4 * n_out);
   return p;
