@@ -37,9 +37,12 @@ constexpr int kPickCap = 1024;  // keys a prompt's selection may keep
 struct ChunkStats {
   double sum;  // of exp(x - max)
   float max;   // -inf: no logit; NaN: bad input
+  float floor; // n_out logits of the chunk are no smaller (-inf: there may be fewer)
   int32_t count;
 };
-constexpr int kPickTight = 256;  // more keys than this are worth a tighter bound
+// More keys than this are worth a tighter bound (12 x 5 beams, first steps among them: 20.6 us a
+// step with 256, 18.5 with 128; 4 x 32 beams: 24.7 with either, 37.2 with 64).
+constexpr int kPickTight = 128;
 
 struct BeamArgs {
   const void *logits;
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(kScanThreads, 7) beam_scan_kernel(const __grid
   float2 *list = a.lists + (int64_t)blockIdx.x * a.cap;
   const float score = a.scores[row];
   if (score == -INFINITY || (a.finished && a.finished[row])) {
-    if (tid == 0) *stats = {0.0, -INFINITY, 0};
+    if (tid == 0) *stats = {0.0, -INFINITY, -INFINITY, 0};
     return;
   }
   const T *x0 = row_of<T>(a, row);
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(kScanThreads, 7) beam_scan_kernel(const __grid
   if (tid == 0) s_count = 0;
   const bool any_bad = __syncthreads_or(bad);
   if (any_bad) {
-    if (tid == 0) *stats = {0.0, NAN, 0};
+    if (tid == 0) *stats = {0.0, NAN, -INFINITY, 0};
     return;
   }
   uint32_t bound = s_bound[0];
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kScanThreads, 7) beam_scan_kernel(const __grid
     cmax = fmaxf(cmax, s_max[w]);
   }
   if (cmax == -INFINITY) {
-    if (tid == 0) *stats = {0.0, -INFINITY, 0};
+    if (tid == 0) *stats = {0.0, -INFINITY, -INFINITY, 0};
     return;
   }
   // Candidates: no smaller than the bound, above -inf.
@@ -310,7 +313,8 @@ __global__ void __launch_bounds__(kScanThreads, 7) beam_scan_kernel(const __grid
     if (lane < kScanWarps && s_max[lane] > -INFINITY)
       t = (double)s_sum[lane] * exp((double)s_max[lane] - (double)cmax);
     t = warp_sum(t);
-    if (lane == 0) *stats = {t, cmax, count};
+    if (lane == 0)
+      *stats = {t, cmax, bound > order_key(-INFINITY) ? key_value(bound) : -INFINITY, count};
   }
 }
 
@@ -440,6 +444,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   __shared__ uint32_t s_again[TABBY_BEAM_MAX], s_need;
   __shared__ double s_part[kMaxHelpers][TABBY_BEAM_MAX];
   __shared__ int s_count;
+  __shared__ uint32_t s_floor;
   const int b = blockIdx.x / a.helpers, helper = blockIdx.x - b * a.helpers, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row0 = b * a.beams, lists = a.beams * a.chunks;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -457,6 +462,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     cluster_wait();
     return;
   }
+  if (tid == 0) s_floor = 0;
   // Log-sum-exps, a warp a beam.
   bool bad = false;
   for (int i = warp; i < a.beams; i += kWarps) {
@@ -513,11 +519,11 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     c.key = s_score[c.beam] + ((double)y.x - s_lse[c.beam]);
     return c;
   };
-  auto list_top = [&](int l) {
+  auto key_of = [&](int l, float x) {  // a logit's of list l
     const int i = l / a.chunks;
-    const float m = stats[l].max;
-    return m > -INFINITY ? s_score[i] + ((double)m - s_lse[i]) : -INFINITY;
+    return x > -INFINITY ? s_score[i] + ((double)x - s_lse[i]) : -INFINITY;
   };
+  auto list_top = [&](int l) { return key_of(l, stats[l].max); };
   auto finished = [&](int i) {
     Cand c;
     c.beam = i;
@@ -585,10 +591,17 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
       if (s_done[i]) keep(finished(i), least);
     __syncthreads();
   };
-  // A bound from the lists' bests; where too much passes it, one from the entries.
-  double top = -INFINITY;
-  for (int l = lane * kWarps + warp; l < lists; l += kThreads) top = fmax(top, list_top(l));
-  double bound = bound_of(top);
+  // A bound from the lists' bests, or the best of the lists' own floors; where too much passes it,
+  // one from the entries.
+  double top = -INFINITY, floor = -INFINITY;
+  for (int l = lane * kWarps + warp; l < lists; l += kThreads) {
+    top = fmax(top, list_top(l));
+    floor = fmax(floor, key_of(l, stats[l].floor));
+  }
+  const uint32_t floors = __reduce_max_sync(0xffffffffu, order_key(__double2float_rd(floor)));
+  if (lane == 0) atomicMax(&s_floor, floors);
+  double bound = bound_of(top);  // its barriers stand behind s_floor
+  bound = fmax(bound, s_floor > order_key(-INFINITY) ? (double)key_value(s_floor) : -INFINITY);
   collect(bound);
   if (s_count > kPickTight) {
     top = -INFINITY;
@@ -736,9 +749,9 @@ ScanPlan scan_plan(int64_t rows, int32_t vocab, int32_t dtype, int32_t n_out) {
   };
   ScanPlan p;
   p.nv = 48 / n;
-  // Few rows: smaller chunks, so that every SM has some (4 rows of 151936: 152 chunks of 6144 leave
-  // no SM two; as 300 of 2048 the scan takes 6.0 us, as 100 it took 7.2).
-  if (rows * chunks(p.nv) < 148) p.nv = 16 / n;
+  // Few rows: smaller chunks, so that more SMs have one (8 rows of 50257 bf16: 11.0 us as 200 chunks
+  // of 2048, 11.7 as 72 of 6144; but 4 rows of 151936: 12.3 as 300, 11.5 as 100).
+  if (rows * chunks(p.nv) < 74) p.nv = 16 / n;
   p.chunks = chunks(p.nv);
   p.cap = std::max(128, 4 * n_out);
   return p;
@@ -754,8 +767,9 @@ cudaError_t launch_beam(const BeamArgs &a, int nv, cudaStream_t q) {
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.batch * a.helpers));
-  // Many lists with many entries: more threads.
-  const int threads = a.beams * a.n_out > 512 ? 1024 : 256;
+  // Many lists with many entries: more threads (4 x 32 beams, 64 out: 37.6 us a step with 256
+  // threads, 24.7 with 1024; 8 x 4, 64 out: 34.2 and 28.7; 32 x 8, 16 out: 34.2 and 53.7).
+  const int threads = a.beams * a.n_out >= 256 ? 1024 : 256;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = q;
   cudaLaunchAttribute attr[2];
@@ -858,7 +872,8 @@ int tabby_beam_step_async(int32_t device, const void *d_logits, int32_t dtype,
   const ScanPlan plan = scan_plan((int64_t)rows, vocab, dtype, n_out);
   a.chunks = plan.chunks;
   a.cap = plan.cap;
-  // Where SMs are left over they help a prompt's CTA with the rare sums in 64 bits.
+  // Where SMs are left over they help a prompt's CTA with the rare sums in 64 bits; otherwise they
+  // cost nothing (32 x 8 beams of 151936: 33.6 us a step without, 34.2 with).
   a.helpers = batch <= 64 ? kMaxHelpers : batch <= 256 ? 2 : 1;
   a.gap = gap_of(vocab);
   a.stats = static_cast<ChunkStats *>(d_workspace);
