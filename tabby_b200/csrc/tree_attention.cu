@@ -72,7 +72,11 @@ struct TreeArgs {
   uint32_t q_and;   // 0 where scale is 0
   float *part_o;    // [2 * workers][dim / 4][prow][4]: unscaled sums
   float2 *part_ml;  // [2 * workers][prow]: m, sum
-  int2 *cuts;       // [items]: slot of the item's first part, its parts (0: not cut)
+  // Items that were cut: sequence, head and row tile (head * mtiles + row tile), the first part's
+  // slot, the parts (0: none). By item where there are no more of them than workers; else by the
+  // worker that has the first part (no worker begins two cut items).
+  int4 *cuts;
+  int32_t items, by_item;
 };
 
 // y / group for a row y < 64 * group (and up to 255 more): with 2^32 / group rounded up the
@@ -158,9 +162,6 @@ struct Walk {
     t = x - t0 - item * nt;
     first = x - t;
     n = min(nt - t, end - x);
-  }
-  __device__ __forceinline__ int64_t item(const TreeArgs &a) const {
-    return ((int64_t)b * a.u.kv_heads + hk) * a.mtiles + mt;
   }
   __device__ __forceinline__ bool more() const { return x < end; }
   __device__ __forceinline__ bool whole() const { return t == 0 && n == nt; }
@@ -457,6 +458,7 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
     uint32_t it = 0;   // tiles of the row tile
     uint32_t itv = 0;  // V tiles of the worker
     bool ok = true;
+    int4 mine = make_int4(0, 0, 0, 0);  // the item that is cut first here
     for (; w.more(); itv += (uint32_t)w.n, w.next(a)) {
       const int64_t L = a.u.lengths[w.b];
       const int row = (w.mt * NS + rt) * kTileM + r;  // of the key/value head's rows
@@ -621,10 +623,12 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
       if (!ok) *err = 1;
       tc_fence_after();
       const bool whole = w.whole();
-      if (tid == 0 && w.t == 0)
-        a.cuts[w.item(a)] =
-            make_int2(2 * blockIdx.x + (w.at_start ? 0 : 1),
-                      whole ? 0 : (int)cut.worker(w.first + w.nt - 1) - (int)blockIdx.x + 1);
+      if (w.t == 0) {
+        int4 c4 = make_int4(w.b, w.hk * a.mtiles + w.mt, 2 * blockIdx.x + (w.at_start ? 0 : 1), 0);
+        if (!whole) c4.w = cut.worker(w.first + w.nt - 1) - (int)blockIdx.x + 1;
+        if (!whole) mine = c4;
+        if (a.by_item && tid == 0) a.cuts[w.b * a.u.kv_heads * a.mtiles + c4.y] = c4;
+      }
       const int64_t slot = 2 * (int64_t)blockIdx.x + (w.at_start ? 0 : 1);
       const float inv = !ok ? NAN : sees == 0 ? 0.f : 1.f / l;
       if (!whole && real) a.part_ml[slot * a.prow + rt * kTileM + r] = make_float2(ok ? m : NAN, l);
@@ -669,11 +673,12 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
       }
       tc_fence_before();
     }
+    if (!a.by_item && tid == 0) a.cuts[blockIdx.x] = mine;
     // Sequences with nothing to attend to: zeros.
     for (int b = blockIdx.x; b < a.u.batch; b += gridDim.x) {
       if (seq_tiles(a, b) != 0) continue;
-      for (int i = tid; i < a.u.kv_heads * a.mtiles; i += 128 * NS)
-        a.cuts[(int64_t)b * a.u.kv_heads * a.mtiles + i] = make_int2(0, 0);
+      for (int i = tid; a.by_item && i < a.u.kv_heads * a.mtiles; i += 128 * NS)
+        a.cuts[b * a.u.kv_heads * a.mtiles + i] = make_int4(0, 0, 0, 0);
       const int64_t per = (int64_t)a.u.heads * dim / 8;
       for (int64_t i = tid; i < a.u.nodes * per; i += 128 * NS) {
         T *out = static_cast<T *>(a.u.out) + (int64_t)b * a.u.out_batch_stride +
@@ -693,37 +698,33 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
   }
 }
 
-// Joins the parts of the items that were cut between workers, with weights 2^(m_i - max m). A
-// part's sums lie as [group of 4 values][row]: a thread takes one place of them, neighbours
-// neighbouring ones, and goes through the parts; `share` threads share out the parts of a place
-// (few places, so that many parts are read at once).
-constexpr int kJoinThreads = 512;
+// Joins the parts of the items that were cut between workers, with weights 2^(m_i - max m); an entry
+// of `cuts` a blockIdx.x. A part's sums lie as [group of 4 values][row]: a thread takes one place
+// of them, neighbours neighbouring ones, and goes through the parts; `share` threads share out the
+// parts of a place.
+constexpr int kJoinThreads = 256;
 
 template <typename T, int NS>
 __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeArgs a,
-                                                                 int64_t items, int share) {
+                                                                 int share) {
   __shared__ int32_t parents[TABBY_TREE_MAX_NODES];
   __shared__ float4 so[kJoinThreads];
   __shared__ float2 sml[kJoinThreads];
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 cut = a.cuts[blockIdx.x];
+  const int n = cut.w;
+  if (n == 0) return;
   const int tid = threadIdx.x, places = kJoinThreads / share;
   const int first = tid / places;  // of the parts
-  const int at = (int)blockIdx.y * places + tid % places;
   const int all = a.u.dim / 4 * a.prow;  // places of a part
-  const int g = at / a.prow, r = at - g * a.prow;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int mt = (int)(item % a.mtiles), hk = (int)(item / a.mtiles % a.u.kv_heads);
-    const int64_t b = item / a.mtiles / a.u.kv_heads;
-    const int2 cut = a.cuts[item];
-    const int64_t L = a.u.lengths[b];
-    int32_t parent = 0;
-    if (tid < a.u.nodes) parent = a.u.parents[b * a.u.parents_stride + tid];
-    const int n = cut.y;
-    if (n == 0) continue;
+  const int64_t b = cut.x;
+  const int hk = cut.y / a.mtiles, mt = cut.y - hk * a.mtiles;
+  const int64_t L = a.u.lengths[b];
+  if (tid < a.u.nodes) parents[tid] = a.u.parents[b * a.u.parents_stride + tid];
+  for (int p0 = blockIdx.y * places; p0 < all; p0 += gridDim.y * places) {
+    const int at = p0 + tid % places, g = at / a.prow, r = at - g * a.prow;
     const int row = mt * NS * kTileM + r, node = div_group(a, row);
     const bool real = at < all && row < a.mrows;
-    __syncthreads();
-    if (tid < a.u.nodes) parents[tid] = parent;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](float m1, float l1, float4 y) {
@@ -738,17 +739,20 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
 #pragma unroll 4
       for (int i = first; i < n; i += share) {
         // The parts behind the first begin their workers' ranges: those have the even slots.
-        const int64_t slot = i == 0 ? cut.x : (cut.x & ~1) + 2 * i;
+        const int64_t slot = i == 0 ? cut.z : (cut.z & ~1) + 2 * i;
         const float2 ml = a.part_ml[slot * a.prow + r];
         add(ml.x, ml.y, reinterpret_cast<const float4 *>(a.part_o)[slot * all + at]);
       }
     }
-    so[tid] = o;
-    sml[tid] = make_float2(m, l);
-    __syncthreads();
+    if (share > 1) {
+      __syncthreads();
+      so[tid] = o;
+      sml[tid] = make_float2(m, l);
+    }
+    __syncthreads();  // the parents are there, too
     if (real && first == 0) {
-      for (int i = 1; i < share; i++) add(sml[i * places + tid].x, sml[i * places + tid].y,
-                                          so[i * places + tid]);
+      for (int i = 1; i < share; i++)
+        add(sml[i * places + tid].x, sml[i * places + tid].y, so[i * places + tid]);
       const float inv = 1.f / l;
       uint2 h = make_uint2(0, 0);
       if (L + node < a.u.entries && tree_sees(parents, node) != 0)
@@ -840,14 +844,13 @@ cudaError_t launch_tree(const TreeArgs &a, const CUtensorMap &mk, const CUtensor
   const cudaError_t err = launch_pdl(tree_kernel<T, DP, NS>, a.workers, Cfg::kThreads, Cfg::kSmem,
                                      s, mk, mv, a);
   if (err != cudaSuccess) return err;
-  const int64_t items = (int64_t)a.u.batch * a.u.kv_heads * a.mtiles;
   const int all = a.u.dim / 4 * a.prow;
-  const int share = all <= 1024 ? 8 : 1;  // a few rows: the parts are shared out
+  const int share = all <= 1024 ? 8 : 1;  // few places: their parts are read by more threads
   const int places = kJoinThreads / share;
   return launch_pdl(tree_join_kernel<T, NS>,
-                    dim3((unsigned)std::min<int64_t>(items, a.workers),
-                         (unsigned)((all + places - 1) / places)),
-                    kJoinThreads, 0, s, a, items, share);
+                    dim3((unsigned)(a.by_item ? a.items : a.workers),
+                         (unsigned)std::min((all + places - 1) / places, a.by_item ? 64 : 8)),
+                    kJoinThreads, 0, s, a, share);
 }
 
 template <typename T>
@@ -870,10 +873,8 @@ int tabby_tree_workspace_bytes(int32_t batch, int32_t nodes, int32_t heads, int3
   if (st) return st;
   if (!bytes) return decode_fail(TABBY_EINVAL, "tree_attention: bytes is NULL");
   const size_t rows = (size_t)std::min<int64_t>((int64_t)nodes * (heads / kv_heads), 2 * kTileM);
-  const size_t items = (size_t)batch * kv_heads *
-                       (((size_t)nodes * (heads / kv_heads) + kTileM - 1) / kTileM);
   *bytes = 2 * (size_t)kMaxWorkers * rows * (sizeof(float2) + (size_t)dim * sizeof(float)) +
-           items * sizeof(int2);
+           kMaxWorkers * sizeof(int4);
   return TABBY_OK;
 }
 
@@ -932,12 +933,14 @@ int tabby_tree_attention_async(int32_t device, const tabby_tree_attention_args *
     return decode_fail(TABBY_EINVAL, "tree_attention: batch * kv_heads * entries is too large");
   t.workers = (int32_t)std::min<double>(std::min((ns == 1 ? 2 : 1) * info.sms, kMaxWorkers),
                                          std::max(1.0, most));
+  t.items = a.batch * a.kv_heads * t.mtiles;  // no more than the tiles
+  t.by_item = t.items <= t.workers;
   t.c = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
   t.q_xor = a.scale < 0.f ? 0x80008000u : 0u;
   t.q_and = a.scale == 0.f ? 0u : 0xffffffffu;
   t.part_o = static_cast<float *>(a.workspace);
   t.part_ml = reinterpret_cast<float2 *>(t.part_o + 2 * (size_t)kMaxWorkers * t.prow * a.dim);
-  t.cuts = reinterpret_cast<int2 *>(t.part_ml + 2 * (size_t)kMaxWorkers * t.prow);
+  t.cuts = reinterpret_cast<int4 *>(t.part_ml + 2 * (size_t)kMaxWorkers * t.prow);
   CUtensorMap mk, mv;
   if (!make_cache_map(&mk, a.k, a, a.k_batch_stride, a.k_head_stride, a.k_entry_stride) ||
       !make_cache_map(&mv, a.v, a, a.v_batch_stride, a.v_head_stride, a.v_entry_stride))
