@@ -130,7 +130,9 @@ TABBY_API int tabby_states_reorder_async(int32_t device, void *const *h_states,
  * t * k_entry_stride (elements), its dim values contiguous; likewise v, q and out (b, j, h).
  * TABBY_BF16 or TABBY_F16; dim a multiple of 8 up to TABBY_TREE_MAX_DIM; heads a multiple of
  * kv_heads; pointers 16-byte aligned and strides multiples of 8 elements.
+ * A cache's axis longer than one has a stride of its own (no shared sequences or heads).
  * parents_stride is the number of ints between the sequences' trees (0: one tree for all).
+ * Should a device-side wait run out of its bound (0.5 s), the outputs it concerns are NaN.
  */
 #define TABBY_TREE_MAX_DIM 128
 typedef struct tabby_tree_attention_args {

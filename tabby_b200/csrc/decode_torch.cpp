@@ -7,6 +7,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cmath>
 #include <optional>
 #include <string>
 #include <vector>
@@ -203,6 +205,11 @@ std::vector<Group> groups_of(const py::object &states, int64_t rows, at::Device 
     }
     at->pointers.push_back(x.data_ptr());
   }
+  std::vector<void *> all;
+  for (const Group &g : groups) all.insert(all.end(), g.pointers.begin(), g.pointers.end());
+  std::sort(all.begin(), all.end());
+  if (std::adjacent_find(all.begin(), all.end()) != all.end())
+    value_error("one of the " + name + " is given twice");
   return groups;
 }
 

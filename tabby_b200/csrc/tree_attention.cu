@@ -39,7 +39,8 @@ namespace {
 
 constexpr int kTileT = 64;        // keys a tile
 constexpr int kTileM = 128;       // query rows a tile (the MMA's M, TMEM's lanes)
-constexpr int kMaxWorkers = 320;  // bounds the workspace: two a SM
+// Workers at most, which bounds the workspace: two an SM, one where two row tiles go together.
+constexpr int max_workers(int64_t mrows) { return mrows > 128 ? 160 : 320; }
 constexpr float kLazy = 8.f;      // the maximum moves when it rises by more than 2^8
 
 // A worker for heads of up to DP values that takes NS row tiles together: they share every K
@@ -845,7 +846,9 @@ cudaError_t launch_tree(const TreeArgs &a, const CUtensorMap &mk, const CUtensor
                                      s, mk, mv, a);
   if (err != cudaSuccess) return err;
   const int all = a.u.dim / 4 * a.prow;
-  const int share = all <= 1024 ? 8 : 1;  // few places: their parts are read by more threads
+  // Few items with few places: their parts are read by more threads. (64 sequences of 8 nodes, 512
+  // items on 296 workers: 54 us with one thread a place, 67 with eight.)
+  const int share = a.by_item && all <= 1024 ? 8 : 1;
   const int places = kJoinThreads / share;
   return launch_pdl(tree_join_kernel<T, NS>,
                     dim3((unsigned)(a.by_item ? a.items : a.workers),
@@ -873,8 +876,8 @@ int tabby_tree_workspace_bytes(int32_t batch, int32_t nodes, int32_t heads, int3
   if (st) return st;
   if (!bytes) return decode_fail(TABBY_EINVAL, "tree_attention: bytes is NULL");
   const size_t rows = (size_t)std::min<int64_t>((int64_t)nodes * (heads / kv_heads), 2 * kTileM);
-  *bytes = 2 * (size_t)kMaxWorkers * rows * (sizeof(float2) + (size_t)dim * sizeof(float)) +
-           kMaxWorkers * sizeof(int4);
+  const size_t workers = (size_t)max_workers((int64_t)nodes * (heads / kv_heads));
+  *bytes = workers * (2 * rows * (sizeof(float2) + (size_t)dim * sizeof(float)) + sizeof(int4));
   return TABBY_OK;
 }
 
@@ -931,7 +934,8 @@ int tabby_tree_attention_async(int32_t device, const tabby_tree_attention_args *
                       (((double)a.entries + kTileT - 1) / kTileT);
   if (most > 2147483647.0)
     return decode_fail(TABBY_EINVAL, "tree_attention: batch * kv_heads * entries is too large");
-  t.workers = (int32_t)std::min<double>(std::min((ns == 1 ? 2 : 1) * info.sms, kMaxWorkers),
+  const int most_workers = max_workers(t.mrows);
+  t.workers = (int32_t)std::min<double>(std::min((ns == 1 ? 2 : 1) * info.sms, most_workers),
                                          std::max(1.0, most));
   t.items = a.batch * a.kv_heads * t.mtiles;  // no more than the tiles
   t.by_item = t.items <= t.workers;
@@ -939,8 +943,8 @@ int tabby_tree_attention_async(int32_t device, const tabby_tree_attention_args *
   t.q_xor = a.scale < 0.f ? 0x80008000u : 0u;
   t.q_and = a.scale == 0.f ? 0u : 0xffffffffu;
   t.part_o = static_cast<float *>(a.workspace);
-  t.part_ml = reinterpret_cast<float2 *>(t.part_o + 2 * (size_t)kMaxWorkers * t.prow * a.dim);
-  t.cuts = reinterpret_cast<int4 *>(t.part_ml + 2 * (size_t)kMaxWorkers * t.prow);
+  t.part_ml = reinterpret_cast<float2 *>(t.part_o + 2 * (size_t)most_workers * t.prow * a.dim);
+  t.cuts = reinterpret_cast<int4 *>(t.part_ml + 2 * (size_t)most_workers * t.prow);
   CUtensorMap mk, mv;
   if (!make_cache_map(&mk, a.k, a, a.k_batch_stride, a.k_head_stride, a.k_entry_stride) ||
       !make_cache_map(&mv, a.v, a, a.v_batch_stride, a.v_head_stride, a.v_entry_stride))

@@ -412,6 +412,8 @@ def test_reorder_refusals(tb):
             tb.reorder_states(states, parents, lengths)
     with pytest.raises(RuntimeError):
         tb.reorder_states([x[:1].expand(6, 2, 5, 8)], p, lens)
+    with pytest.raises(ValueError):
+        tb.reorder_states([x, x], p, lens)
     with pytest.raises(RuntimeError):
         tb.reorder_states([filled((65, 4), torch.int32, 1)], random_parents(1, 65, 1))
     tb.reorder_states([], p)
@@ -703,6 +705,8 @@ def test_tree_attention_refusals(tb):
         n = a[0].shape[1]
         with pytest.raises(RuntimeError):
             tb.tree_attention(*a, lengths, random_trees(2, n, 1))
+    with pytest.raises(RuntimeError):  # one cache for all sequences
+        tb.tree_attention(q, k[:1].expand(2, 2, 40, 64), v, lengths, parents)
     odd = torch.zeros(2, 2, 40, 68, dtype=torch.bfloat16, device="cuda")[..., :64]
     with pytest.raises(ValueError):
         tb.tree_attention(q, odd, v, lengths, parents)
@@ -824,7 +828,7 @@ def test_tree_accept_refusals(tb):
     for a in ((z[:1], z, z, lens), (z, z.long(), z, lens), (z, z, z[:, :3], lens),
               (z, z, z, lens[:1]), (z.cpu(), z, z, lens), (z, z, z, lens, [c[:1]]),
               (z, z, z, lens, [c[:, 0]]), (z, z, z, lens, [c, c[:, :, :8]]),
-              (z, z, z, lens, [c.cpu()])):
+              (z, z, z, lens, [c.cpu()]), (z, z, z, lens, [c, c])):
         with pytest.raises((TypeError, ValueError)):
             tb.tree_accept(*a)
     w = torch.zeros(2, 65, dtype=torch.int32, device="cuda")
@@ -959,6 +963,35 @@ def test_drafted_decoding_with_the_sampler(tb):
             best = int(logits.argmax())
             got = texts[b][i]
             assert got == best or logits[best] - logits[got] <= tol[best] + tol[got]
+
+
+def test_calls_side_by_side(tb):
+    """All operators at once on streams of their own, with other work between."""
+    x, scores = beam_inputs(8, 4, 30000, "bf16", seed=3)
+    q, k, v = attention_inputs(4, 9, 8, 2, 64, 900, "bf16", 4)
+    lengths = torch.tensor([800, 3, 500, 64], dtype=torch.int32, device="cuda")
+    parents = random_trees(4, 9, 5)
+    state = filled((32, 2, 40, 64), torch.bfloat16, 6)
+    moves = random_parents(8, 4, 7)
+    want_beam, want_tree = tb.beam_step(x, scores, 8), tb.tree_attention(q, k, v, lengths, parents)
+    want_state = state.clone()
+    for _ in range(5):
+        want_state = plain_reorder(want_state, moves)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    beams, trees = [], []
+    for _ in range(5):
+        with torch.cuda.stream(streams[0]):
+            beams.append(tb.beam_step(x, scores, 8))
+        with torch.cuda.stream(streams[1]):
+            trees.append(tb.tree_attention(q, k, v, lengths, parents))
+        with torch.cuda.stream(streams[2]):
+            tb.reorder_states([state], moves)
+    torch.cuda.synchronize()
+    for r in beams:
+        assert all(torch.equal(a, b) for a, b in zip(want_beam, r))
+    assert all(torch.equal(want_tree, o) for o in trees)
+    assert torch.equal(state.view(torch.int16), want_state.view(torch.int16))
 
 
 def test_tensors_on_a_device_that_is_not_current(tb):
