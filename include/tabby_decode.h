@@ -45,7 +45,8 @@ TABBY_API const char *tabby_decode_last_error(void);
  * s = scores[b][i] and logits x[v], v < vocab:
  *   key(i, v) = s + x[v] - log(sum_u exp(x[u]))          (compared in 64 bits)
  * and the n_out continuations with the largest keys are written in falling order, ties to
- * the lower (beam, token); among one beam's continuations the logits themselves decide. Of prompt b, output j:
+ * the lower (beam, token); among one beam's continuations the logits themselves decide. Of
+ * prompt b, output j:
  *   next_scores = key rounded to f32, parents = i, tokens = v,
  *   next_finished = 1 where beam i was finished or v == eos_id.
  * - A logit of -inf is a banned token: it is no candidate. Any finite logit is one.
@@ -62,7 +63,7 @@ TABBY_API const char *tabby_decode_last_error(void);
  * Scores are exact to (3 ln(vocab) + 24) 2^-24 and their rounding to f32; parents and tokens are
  * those of 64-bit keys.
  * 1 <= beams <= TABBY_BEAM_MAX, 1 <= n_out <= TABBY_BEAM_MAX_OUT, 1 <= vocab <= 2^30,
- * beams * vocab < 2^31.
+ * beams * vocab < 2^31; batch * beams * vocab below 2^42 or so (a launch's 2^31 blocks).
  * d_workspace: tabby_beam_workspace_bytes bytes, 16-byte aligned.
  */
 #define TABBY_BEAM_MAX 64

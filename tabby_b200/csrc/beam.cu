@@ -360,10 +360,13 @@ struct CandTable {
   }
 };
 
+// (Aligned, like the wait: the warp has to be converged, whatever branch stood before.)
 __device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The address of the first CTA's copy of a shared variable, for the cluster's other CTAs.
@@ -445,7 +448,8 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   __shared__ double s_part[kMaxHelpers][TABBY_BEAM_MAX];
   __shared__ int s_count;
   __shared__ uint32_t s_floor;
-  const int b = blockIdx.x / a.helpers, helper = blockIdx.x - b * a.helpers, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.x / a.helpers, helper = blockIdx.x - b * a.helpers;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row0 = b * a.beams, lists = a.beams * a.chunks;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const ChunkStats *stats = a.stats + (int64_t)row0 * a.chunks;
@@ -729,10 +733,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   }
   for (int j = tid; j < a.n_out; j += kThreads)
     write(j, j >= n, j < n ? s_cand.get(s_order[j]) : Cand());
-  if (!again && !many) {
-    __syncwarp();
-    cluster_wait();  // the others have read the word
-  }
+  if (!again && !many) cluster_wait();  // the others have read the word
 }
 
 // Chunks of a row: at most 128 threads' worth of pieces each.
@@ -796,7 +797,8 @@ int check_sizes(int32_t batch, int32_t beams, int32_t vocab, int32_t n_out) {
   if ((int64_t)beams * vocab > INT32_MAX)
     return decode_fail(TABBY_EINVAL, "beam_step: beams * vocab must be below 2^31");
   for (int32_t dtype : {TABBY_F32, TABBY_BF16, TABBY_F16})
-    if ((int64_t)batch * beams > INT32_MAX / scan_plan((int64_t)batch * beams, vocab, dtype, n_out).chunks)
+    if ((int64_t)batch * beams >
+        INT32_MAX / scan_plan((int64_t)batch * beams, vocab, dtype, n_out).chunks)
       return decode_fail(TABBY_EINVAL, "beam_step: batch * beams * vocab is too large");
   return TABBY_OK;
 }

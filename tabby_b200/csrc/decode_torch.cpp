@@ -68,13 +68,15 @@ void *stream_of(at::Device device) {
 }
 
 int32_t size32(int64_t n, const char *what) {
-  if (n > INT32_MAX) value_error(std::string(what) + " is too large");
+  if (n > INT32_MAX || n < INT32_MIN)
+    value_error(std::string(what) + " is out of range: " + std::to_string(n));
   return (int32_t)n;
 }
 
 // -1 for a type that the library does not know.
 int32_t type_of(at::ScalarType t) {
-  return t == at::kFloat ? TABBY_F32 : t == at::kBFloat16 ? TABBY_BF16 : t == at::kHalf ? TABBY_F16 : -1;
+  return t == at::kFloat ? TABBY_F32 : t == at::kBFloat16 ? TABBY_BF16
+                                   : t == at::kHalf ? TABBY_F16 : -1;
 }
 
 py::tuple beam_step(Tensor logits, Tensor scores, std::optional<int64_t> n_out_or,
@@ -316,6 +318,9 @@ py::tuple tree_accept(const Tensor &sampled, Tensor tokens, Tensor parents, Tens
   const std::vector<Group> groups = groups_of(caches, batch, device, "caches");
   if (groups.size() > 1) value_error("the caches must share one layout");
   tabby_state_layout l = {};
+  // (Without a cache no slot lies past the end: one without an entry is not the same.)
+  if (groups.empty() && batch > 0 && py::len(caches) > 0)
+    value_error("the caches must not be empty");
   if (!groups.empty()) l = layout_of(groups[0].shape, groups[0].stride, groups[0].size, true);
   Tensor path = fresh({batch, nodes}, at::kInt, device);
   Tensor counts = fresh({batch}, at::kInt, device);

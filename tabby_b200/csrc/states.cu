@@ -208,9 +208,10 @@ tabby_state_layout merged(tabby_state_layout l) {
   return l;
 }
 
-// Columns a thread, by the values it holds for each.
+// Columns a thread, by the bytes of registers that it holds for each (4 at least a value).
 constexpr int columns_of(int w, int k) {
-  return w * k <= 64 ? 4 : w * k <= 128 ? 2 : 1;
+  const int bytes = std::max(w, 4) * k;
+  return bytes <= 64 ? 4 : bytes <= 128 ? 2 : 1;
 }
 
 template <int W, int K>

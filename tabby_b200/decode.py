@@ -2,7 +2,8 @@
 
 The calls of include/tabby_decode.h on torch tensors. All of them are asynchronous on the
 current stream of the tensors' device, take and give device tensors, allocate through
-PyTorch (so they can be captured in a CUDA graph) and keep nothing between calls.
+PyTorch (so they can be captured in a CUDA graph) and keep nothing between calls. They take no
+part in autograd.
 
 Beam search, one step:
 

@@ -5,8 +5,9 @@ Tolerances. u = 2^-24.
 - beam scores: a term exp(x - max) of the sum has relative error at most (3 |x - max| + 4) u
   (the difference, its product with log2 e, the constant; ex2's 4 u). Weighted with the
   probabilities the |x - max| average to at most ln V. Summation in fp32 adds at most 20 u
-  (short runs, then a tree; the rest is done in 64 bits). So |score - exact| <= (3 ln V + 24) u, plus half a step
-  of the fp32 result, u |score|. Parents, tokens and flags have to be equal.
+  (short runs, then a tree; the rest is done in 64 bits). So |score - exact| <=
+  (3 ln V + 24) u, plus half a step of the fp32 result, u |score|. Parents, tokens and flags
+  have to be equal.
 - attention: out is rounded to its type (half a step h relative), the weights p once to it
   (h relative each, A = sum p |v|), a score's fp32 dot product is off by at most
   (dim + 4) 2^-23 S, S the largest scale * sum |q| |k|, which moves the weights by that twice;
@@ -14,6 +15,9 @@ Tolerances. u = 2^-24.
   (4 + 3 * 2 S) u, twice.
 """
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -267,6 +271,8 @@ def test_beam_step_refusals(tb):
             tb.beam_step(x, scores, **bad)
     with pytest.raises(RuntimeError):
         tb.beam_step(x, scores, finished=torch.zeros(2, 3, dtype=torch.bool, device="cuda"))
+    with pytest.raises(ValueError):
+        tb.beam_step(x, scores, eos_id=3 - 2 ** 32)
     with pytest.raises(ValueError):
         tb.beam_step(x[0], scores)
     with pytest.raises(ValueError):
@@ -828,7 +834,8 @@ def test_tree_accept_refusals(tb):
     for a in ((z[:1], z, z, lens), (z, z.long(), z, lens), (z, z, z[:, :3], lens),
               (z, z, z, lens[:1]), (z.cpu(), z, z, lens), (z, z, z, lens, [c[:1]]),
               (z, z, z, lens, [c[:, 0]]), (z, z, z, lens, [c, c[:, :, :8]]),
-              (z, z, z, lens, [c.cpu()]), (z, z, z, lens, [c, c])):
+              (z, z, z, lens, [c.cpu()]), (z, z, z, lens, [c, c]),
+              (z, z, z, lens, [c[:, :, :0]])):
         with pytest.raises((TypeError, ValueError)):
             tb.tree_accept(*a)
     w = torch.zeros(2, 65, dtype=torch.int32, device="cuda")
@@ -963,6 +970,48 @@ def test_drafted_decoding_with_the_sampler(tb):
             best = int(logits.argmax())
             got = texts[b][i]
             assert got == best or logits[best] - logits[got] <= tol[best] + tol[got]
+
+
+FIRST_CAPTURE = """
+import torch
+import tabby_b200 as tb
+
+g = torch.Generator(device="cuda").manual_seed(1)
+x = torch.randn(2, 4, 9000, device="cuda", generator=g)
+s = torch.zeros(2, 4, device="cuda")
+q = torch.randn(2, 5, 8, 64, device="cuda", generator=g).bfloat16()
+kv = torch.randn(2, 2, 2, 300, 64, device="cuda", generator=g).bfloat16()
+lengths = torch.tensor([200, 7], dtype=torch.int32, device="cuda")
+tree = torch.tensor([-1, 0, 0, 1, 1], dtype=torch.int32, device="cuda")
+tokens = torch.tensor([[9, 1, 2, 3, 4]] * 2, dtype=torch.int32, device="cuda")
+sampled = torch.tensor([[2, 0, 0, 0, 5], [1, 4, 0, 0, 6]], dtype=torch.int32, device="cuda")
+state = torch.arange(8 * 6, device="cuda").view(8, 6)
+kv2, state2 = kv.clone(), state.clone()
+
+
+def run(kv, state):
+    beams = tb.beam_step(x, s)
+    tb.reorder_states([state], beams.parents)
+    out = tb.tree_attention(q, kv[0], kv[1], lengths, tree)
+    return (*beams, out, *tb.tree_accept(sampled, tokens, tree, lengths, kv), kv, state)
+
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run(kv, state)
+graph.replay()
+want = run(kv2, state2)
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("same")
+"""
+
+
+def test_first_calls_captured(tb):
+    """A process whose first calls of all are captured into a graph."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", FIRST_CAPTURE], cwd=root, capture_output=True,
+                       text=True, timeout=240)
+    assert p.returncode == 0 and "same" in p.stdout, p.stderr[-2000:]
 
 
 def test_calls_side_by_side(tb):
