@@ -846,13 +846,17 @@ cudaError_t launch_tree(const TreeArgs &a, const CUtensorMap &mk, const CUtensor
                                      s, mk, mv, a);
   if (err != cudaSuccess) return err;
   const int all = a.u.dim / 4 * a.prow;
-  // Few items with few places: their parts are read by more threads. (64 sequences of 8 nodes, 512
-  // items on 296 workers: 54 us with one thread a place, 67 with eight.)
-  const int share = a.by_item && all <= 1024 ? 8 : 1;
+  // Items of many parts: up to eight threads share a place's parts, as far as all of them run at
+  // once. (8 sequences of 26 nodes, 40 items of 7 parts: 21.9 us a call with four, 24.7 with one; 64
+  // sequences of 8 nodes, 512 items on 296 workers: 54 with one, 67 with eight.)
+  int share = 1;
+  while (a.by_item && share < 8 && 2 * share * a.items <= a.workers &&
+         (int64_t)2 * share * a.items * all <= (int64_t)a.workers * 1024)
+    share *= 2;
   const int places = kJoinThreads / share;
   return launch_pdl(tree_join_kernel<T, NS>,
                     dim3((unsigned)(a.by_item ? a.items : a.workers),
-                         (unsigned)std::min((all + places - 1) / places, a.by_item ? 64 : 8)),
+                         (unsigned)std::min((all + places - 1) / places, a.by_item ? 64 * share : 8)),
                     kJoinThreads, 0, s, a, share);
 }
 
