@@ -40,8 +40,9 @@ struct ChunkStats {
   float floor; // n_out logits of the chunk are no smaller (-inf: there may be fewer)
   int32_t count;
 };
-// More keys than this are worth a tighter bound (12 x 5 beams, first steps among them: 20.6 us a
-// step with 256, 18.5 with 128; 4 x 32 beams: 24.7 with either, 37.2 with 64).
+// More keys than this are worth a tighter bound (12 x 5 beams, first steps among them, before
+// the ranking went without branches: 20.6 us a step with 256, 18.5 with 128; 4 x 32 beams: the same
+// with either, half as much again with 64).
 constexpr int kPickTight = 128;
 
 struct BeamArgs {
@@ -369,16 +370,20 @@ __device__ __forceinline__ void cluster_wait() {
   __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The address of the first CTA's copy of a shared variable, for the cluster's other CTAs.
-__device__ __forceinline__ uint32_t in_first_cta(const void *p) {
+// The address of a shared variable's copy in a CTA of the cluster.
+__device__ __forceinline__ uint32_t in_cta(const void *p, int cta) {
   uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr(p)));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(cta));
   return r;
 }
+__device__ __forceinline__ uint32_t in_first_cta(const void *p) { return in_cta(p, 0); }
 __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void store_cluster(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
@@ -437,11 +442,9 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   constexpr int kWarps = kThreads / 32;
   __shared__ double s_lse[TABBY_BEAM_MAX], s_score[TABBY_BEAM_MAX];
   __shared__ double s_bound[kWarps];
-  __shared__ int s_sums[kWarps];
   __shared__ CandTable s_cand;
   __shared__ int16_t s_order[kPickCap];
   __shared__ int s_rank[kPickCap];
-  int *s_end = s_rank;  // of the threads' lists, before anything is ranked
   __shared__ float s_rowmax[TABBY_BEAM_MAX];
   __shared__ uint8_t s_done[TABBY_BEAM_MAX];
   __shared__ uint32_t s_again[TABBY_BEAM_MAX], s_need;
@@ -451,21 +454,29 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   const int b = blockIdx.x / a.helpers, helper = blockIdx.x - b * a.helpers;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row0 = b * a.beams, lists = a.beams * a.chunks;
+  cluster_arrive();  // all of the cluster run once this is complete
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const ChunkStats *stats = a.stats + (int64_t)row0 * a.chunks;
   if (helper > 0) {  // waits for the first CTA's word
+    cluster_wait();
     cluster_arrive();
     cluster_wait();
-    if (load_cluster(in_first_cta(&s_need)))
-      for (int i = 0; i < a.beams; i++)
-        if (load_cluster(in_first_cta(&s_again[i])))
-          share_sum<T, kThreads>(a, row0 + i,
-                                 __uint_as_float(load_cluster(in_first_cta(&s_rowmax[i]))),
-                                 helper, s_bound, in_first_cta(&s_part[helper][i]));
+    if (!s_need) return;
+    for (int i = 0; i < a.beams; i++)
+      if (load_cluster(in_first_cta(&s_again[i])))
+        share_sum<T, kThreads>(a, row0 + i,
+                               __uint_as_float(load_cluster(in_first_cta(&s_rowmax[i]))), helper,
+                               s_bound, in_first_cta(&s_part[helper][i]));
     cluster_arrive();
     cluster_wait();
     return;
   }
+  // The word to the others, whether they are needed; a cluster_wait() stands behind it.
+  auto tell = [&](uint32_t need) {
+    cluster_wait();
+    if (tid > 0 && tid < a.helpers) store_cluster(in_cta(&s_need, tid), need);
+    cluster_arrive();
+  };
   if (tid == 0) s_floor = 0;
   // Log-sum-exps, a warp a beam.
   bool bad = false;
@@ -505,19 +516,15 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   };
   if (tid == 0) a.status[b] = bad ? TABBY_EINPUT : TABBY_OK;
   if (bad) {
+    tell(0);
     for (int j = tid; j < a.n_out; j += kThreads) write(j, true, Cand());
-    if (tid == 0) s_need = 0;
-    cluster_arrive();
     cluster_wait();
-    cluster_arrive();
-    cluster_wait();  // the others have read the word
     return;
   }
-  // Entry e of list l, a list's best key.
-  auto entry = [&](int l, int e) {
-    const float2 y = a.lists[((int64_t)row0 * a.chunks + l) * a.cap + e];
+  // A beam's entry of a list, a list's best key.
+  auto entry = [&](int beam, float2 y) {
     Cand c;
-    c.beam = l / a.chunks;
+    c.beam = beam;
     c.token = __float_as_int(y.y);
     c.x = y.x;
     c.key = s_score[c.beam] + ((double)y.x - s_lse[c.beam]);
@@ -552,36 +559,60 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     const int at = atomicAdd(&s_count, 1);
     if (at < kPickCap) s_cand.put(at, c);
   };
-  // Goes over the entries of the lists whose best reaches `least`: a thread looks at a list,
-  // their entries are laid end to end and then shared out evenly.
+  // Goes over the entries of the lists whose best reaches `least`, four entries a lane on their way
+  // at a time. A warp looks at 32 lists. Where lists are long (the CTAs of 1024 threads) its lanes
+  // then go through one after the other; where they are short they are laid end to end. (4 x 32
+  // beams, 64 out: 22.0 us a step one after the other, 24.7 end to end; 2 x 4 beams, 8 out: 11.7
+  // and 10.3.)
   auto each_entry = [&](double least, auto use) {
-    for (int l0 = 0; l0 < lists; l0 += kThreads) {
-      const int l = l0 + tid;
-      int count = l < lists ? stats[l].count : 0;
-      if (count > 0 && !(list_top(l) >= least)) count = 0;
-      int end = count;  // inclusive over the threads
+    for (int l0 = warp; l0 < lists; l0 += 32 * kWarps) {
+      const int mine = l0 + lane * kWarps;
+      int count = mine < lists ? stats[mine].count : 0;
+      if (count > 0 && !(list_top(mine) >= least)) count = 0;
+      if constexpr (kThreads > 256) {
+        for (unsigned in = __ballot_sync(0xffffffffu, count > 0); in; in &= in - 1) {
+          const int f = __ffs(in) - 1, n = __shfl_sync(0xffffffffu, count, f);
+          const int l = l0 + f * kWarps, beam = l / a.chunks;
+          const float2 *list = a.lists + ((int64_t)row0 * a.chunks + l) * a.cap;
+          for (int e = lane; e < n; e += 128) {
+            float2 y[4];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, end, o);
-        if (lane >= o) end += y;
-      }
-      __syncthreads();
-      if (lane == 31) s_sums[warp] = end;
-      __syncthreads();
-      int all = 0;
+            for (int k = 0; k < 4; k++) y[k] = list[min(e + 32 * k, n - 1)];
 #pragma unroll
-      for (int w = 0; w < kWarps; w++) {
-        if (w < warp) end += s_sums[w];
-        all += s_sums[w];
-      }
-      s_end[tid] = end;
-      __syncthreads();
-      for (int f = tid; f < all; f += kThreads) {
-        int lo = 0;  // the first list that ends behind f
+            for (int k = 0; k < 4; k++)
+              if (e + 32 * k < n) use(entry(beam, y[k]));
+          }
+          __syncwarp();
+        }
+      } else {
+        const int beam = mine / a.chunks;
+        int end = count;  // inclusive over the lanes
 #pragma unroll
-        for (int o = kThreads / 2; o > 0; o >>= 1)
-          if (s_end[lo + o - 1] <= f) lo += o;
-        use(entry(l0 + lo, f - (lo > 0 ? s_end[lo - 1] : 0)));
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, end, o);
+          if (lane >= o) end += y;
+        }
+        const int all = __shfl_sync(0xffffffffu, end, 31);
+        for (int f0 = 0; f0 < all; f0 += 128) {
+          float2 y[4];
+          int of[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            if (f0 + 32 * k >= all) break;  // the whole warp
+            const int f = min(f0 + 32 * k + lane, all - 1);
+            int lo = 0;  // the first list that ends behind f
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+              if (__shfl_sync(0xffffffffu, end, lo + o - 1) <= f) lo += o;
+            const int e = f - __shfl_sync(0xffffffffu, end - count, lo);
+            y[k] = a.lists[((int64_t)row0 * a.chunks + l0 + lo * kWarps) * a.cap + e];
+            of[k] = __shfl_sync(0xffffffffu, beam, lo);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (f0 + 32 * k + lane < all) use(entry(of[k], y[k]));
+          __syncwarp();
+        }
       }
     }
   };
@@ -616,8 +647,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   }
   // The lse of the marked beams in 64 bits, from all their logits, with the cluster's help.
   auto refine = [&]() {
-    if (tid == 0) s_need = 1;
-    cluster_arrive();
+    tell(1);
     cluster_wait();
     for (int i = 0; i < a.beams; i++)
       if (s_again[i])
@@ -684,8 +714,30 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     __syncthreads();
   }
   const int n = s_count;
-  auto rank = [&]() {  // s_order[j]: the candidate of rank j; a few threads a candidate
-    const int parts = max(1, kThreads / max(n, 1));
+  // 1 where candidate 2 stands before; without branches, of which each costs tens of cycles.
+  auto before = [](int64_t key2, uint64_t tie2, int32_t token2, int64_t key, uint64_t tie,
+                   int32_t token) {
+    const unsigned less = (unsigned)(tie2 < tie) |
+                          ((unsigned)(tie2 == tie) & (unsigned)(token2 < token));
+    return (int)((unsigned)(key2 > key) | ((unsigned)(key2 == key) & less));
+  };
+  auto rank = [&]() {  // s_order[j]: the candidate of rank j
+    if (n <= 32) {  // a warp, a candidate a lane
+      if (warp == 0) {
+        const int me = min(lane, max(n, 1) - 1);
+        const int64_t key = s_cand.key[me];
+        const uint64_t tie = s_cand.tie[me];
+        const int32_t token = s_cand.token[me];
+        int r = 0;
+        for (int k = 0; k < n; k++)
+          r += before(__shfl_sync(0xffffffffu, key, k), __shfl_sync(0xffffffffu, tie, k),
+                      __shfl_sync(0xffffffffu, token, k), key, tie, token);
+        if (lane < n) s_order[r] = (int16_t)lane;
+      }
+      __syncthreads();
+      return;
+    }
+    const int parts = max(1, kThreads / n);  // a few threads a candidate
     for (int i = tid; i < n; i += kThreads) s_rank[i] = 0;
     __syncthreads();
     for (int i = tid; i < n * parts; i += kThreads) {
@@ -694,10 +746,9 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
       const uint64_t tie = s_cand.tie[me];
       const int32_t token = s_cand.token[me];
       int r = 0;
-      for (int k = p; k < n; k += parts) {
-        const bool less = s_cand.tie[k] < tie || (s_cand.tie[k] == tie && s_cand.token[k] < token);
-        r += s_cand.key[k] > key || (s_cand.key[k] == key && less) ? 1 : 0;
-      }
+#pragma unroll 4
+      for (int k = p; k < n; k += parts)
+        r += before(s_cand.key[k], s_cand.tie[k], s_cand.token[k], key, tie, token);
       if (r) atomicAdd(&s_rank[me], r);
     }
     __syncthreads();
@@ -725,15 +776,10 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     __syncthreads();
     rank();
   }
-  if (!again && !many) {
-    if (tid == 0) s_need = 0;
-    cluster_arrive();
-    cluster_wait();
-    cluster_arrive();
-  }
+  if (!again && !many) tell(0);
   for (int j = tid; j < a.n_out; j += kThreads)
     write(j, j >= n, j < n ? s_cand.get(s_order[j]) : Cand());
-  if (!again && !many) cluster_wait();  // the others have read the word
+  if (!again && !many) cluster_wait();
 }
 
 // Chunks of a row: at most 128 threads' worth of pieces each.
