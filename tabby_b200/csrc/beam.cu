@@ -40,9 +40,8 @@ struct ChunkStats {
   float floor; // n_out logits of the chunk are no smaller (-inf: there may be fewer)
   int32_t count;
 };
-// More keys than this are worth a tighter bound (12 x 5 beams, first steps among them, before
-// the ranking went without branches: 20.6 us a step with 256, 18.5 with 128; 4 x 32 beams: the same
-// with either, half as much again with 64).
+// More keys than this are worth a tighter bound (12 x 5 beams, first steps among them: 16.0 us a
+// step with 256, 15.8 with 128, 16.9 with 64; 4 x 32 beams: 22.0, 22.0 and 30.7).
 constexpr int kPickTight = 128;
 
 struct BeamArgs {
@@ -796,8 +795,8 @@ ScanPlan scan_plan(int64_t rows, int32_t vocab, int32_t dtype, int32_t n_out) {
   };
   ScanPlan p;
   p.nv = 48 / n;
-  // Few rows: smaller chunks, so that more SMs have one (8 rows of 50257 bf16: 11.0 us as 200 chunks
-  // of 2048, 11.7 as 72 of 6144; but 4 rows of 151936: 12.3 as 300, 11.5 as 100).
+  // Few rows: smaller chunks, so that more SMs have one (8 rows of 50257 bf16: 10.5 us as 200
+  // chunks of 2048, 11.7 as 72 of 6144; but 4 rows of 151936: 11.7 as 300, 11.0 as 100).
   if (rows * chunks(p.nv) < 74) p.nv = 16 / n;
   p.chunks = chunks(p.nv);
   p.cap = std::max(128, 4 * n_out);
@@ -814,8 +813,8 @@ cudaError_t launch_beam(const BeamArgs &a, int nv, cudaStream_t q) {
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.batch * a.helpers));
-  // Many lists with many entries: more threads (4 x 32 beams, 64 out: 37.6 us a step with 256
-  // threads, 24.7 with 1024; 8 x 4, 64 out: 34.2 and 28.7; 32 x 8, 16 out: 34.2 and 53.7).
+  // Many lists with many entries: more threads (4 x 32 beams, 64 out: 33.5 us a step with 256
+  // threads, 22.0 with 1024; 8 x 4, 64 out: 32.1 and 23.3; 32 x 8, 16 out: 34.2 and 52.0).
   const int threads = a.beams * a.n_out >= 256 ? 1024 : 256;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = q;
@@ -921,7 +920,7 @@ int tabby_beam_step_async(int32_t device, const void *d_logits, int32_t dtype,
   a.chunks = plan.chunks;
   a.cap = plan.cap;
   // Where SMs are left over they help a prompt's CTA with the rare sums in 64 bits; otherwise they
-  // cost nothing (32 x 8 beams of 151936: 33.6 us a step without, 34.2 with).
+  // cost nothing (32 x 8 beams of 151936: 34.0 us a step without, 34.2 with).
   a.helpers = batch <= 64 ? kMaxHelpers : batch <= 256 ? 2 : 1;
   a.gap = gap_of(vocab);
   a.stats = static_cast<ChunkStats *>(d_workspace);
