@@ -11,7 +11,10 @@
 namespace tabby {
 namespace {
 
-constexpr unsigned long long kWaitNs = 500000000ull;  // a bounded wait gives up after 0.5 s
+#ifndef TABBY_WAIT_NS
+#define TABBY_WAIT_NS 500000000ull
+#endif
+constexpr unsigned long long kWaitNs = TABBY_WAIT_NS;  // a bounded wait gives up after 0.5 s
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) {
   return (uint32_t)__cvta_generic_to_shared(p);

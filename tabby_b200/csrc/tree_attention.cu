@@ -43,6 +43,18 @@ constexpr int kTileM = 128;       // query rows a tile (the MMA's M, TMEM's lane
 constexpr int max_workers(int64_t mrows) { return mrows > 128 ? 160 : 320; }
 constexpr float kLazy = 8.f;      // the maximum moves when it rises by more than 2^8
 
+// Builds that check themselves (-DTABBY_CHECKS=1) can make waits of one sequence's tiles run out
+// (tabby_debug_tree): its value tiles are never loaded, or the first issuer gives up behind a
+// product of it that it has just issued. Every wait is bounded, so the kernel returns all the same.
+// They count the CTAs that would give their TMEM back with a product on its way.
+#ifdef TABBY_CHECKS
+struct TreeChecks {
+  int withhold, give_up;  // sequences, -1: none
+  int in_flight;
+};
+__device__ TreeChecks g_tree_checks = {-1, -1, 0};
+#endif
+
 // A worker for heads of up to DP values that takes NS row tiles together: they share every K
 // and V tile. One row tile: two workers an SM; two: one.
 template <int DP, int NS>
@@ -348,6 +360,12 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
                       const CUtensorMap *map, int tile) {
         const uint32_t s = i % kStages;
         if (!mb_wait(&empty[s], ((i / kStages) & 1u) ^ 1u)) return false;
+#ifdef TABBY_CHECKS
+        if (full == vfull && w.b == g_tree_checks.withhold) {
+          i++;
+          return true;
+        }
+#endif
         mb_arrive_expect(&full[s], (uint32_t)Cfg::kKv);
         for (int d = 0; d < Cfg::kBlocks; d++)
           tma_load_4d(ring + s * Cfg::kKv + d * kTileT * 128, map, d * 64, tile * kTileT, w.hk,
@@ -439,12 +457,18 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
         __syncwarp();
         iv++;
         io++;
+#ifdef TABBY_CHECKS
+        if (r == 0 && w.b == g_tree_checks.give_up) ok = false;
+#endif
       }
     }
     if (!ok) *err = 1;
-    if (elect_one()) mma_commit(drain);  // every product is done before TMEM goes
+    // Every product is done before the tiles and TMEM go, also where a wait ran out, here or in
+    // another warp: what was issued ends by itself. (Whichever issuer comes last waits for all.)
+    if (elect_one()) mma_commit(drain);
     __syncwarp();
-    wait_or(drain, 0, err);
+    mb_wait(drain, 0);
+    __syncwarp();
   } else {
     // ---- softmax: four warps a row tile, one row a thread ----
     const int rt = warp >> 2, r = tid & 127;  // row tile and row in it
@@ -691,6 +715,19 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
   }
   tc_fence_before();
   __syncthreads();
+#ifdef TABBY_CHECKS
+  if (tid == 0) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], 0;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(drain))
+        : "memory");
+    if (!done) atomicAdd(&g_tree_checks.in_flight, 1);
+  }
+#endif
   if (warp == 4 * NS + 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
@@ -959,5 +996,19 @@ int tabby_tree_attention_async(int32_t device, const tabby_tree_attention_args *
   if (err != cudaSuccess) return decode_cuda_fail(err, "tree_attention launch");
   return TABBY_OK;
 }
+
+#ifdef TABBY_CHECKS
+// Sets the sequences whose tiles are withheld (-1: none) and gives the count of CTAs.
+TABBY_API int tabby_debug_tree(int32_t withhold, int32_t give_up, int32_t *in_flight) {
+  tabby::TreeChecks c;
+  cudaError_t err = cudaMemcpyFromSymbol(&c, tabby::g_tree_checks, sizeof(c));
+  if (err == cudaSuccess) {
+    *in_flight = c.in_flight;
+    c = {withhold, give_up, 0};
+    err = cudaMemcpyToSymbol(tabby::g_tree_checks, &c, sizeof(c));
+  }
+  return (int)err;
+}
+#endif
 
 }  // extern "C"
