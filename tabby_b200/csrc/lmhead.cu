@@ -144,6 +144,17 @@ __device__ __forceinline__ uint64_t merge_pending(unsigned long long *tab, int r
   return __shfl_sync(0xffffffffu, a1, 31);
 }
 
+// Builds that check themselves (-DTABBY_CHECKS=1) can let the issuer of one tile give up behind
+// products that it has just issued (tabby_debug_lmhead). They count the CTAs that would give
+// their TMEM back with products on their way.
+#ifdef TABBY_CHECKS
+struct LmChecks {
+  int give_up;  // a tile, -1: none
+  int in_flight;
+};
+__device__ LmChecks g_lm_checks = {-1, 0};
+#endif
+
 template <int KL>
 __global__ void __launch_bounds__(kLmThreads, 1)
     lmhead_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
@@ -164,7 +175,8 @@ __global__ void __launch_bounds__(kLmThreads, 1)
   uint64_t *wfull = bars, *wempty = bars + kWMax;
   uint64_t *afull = bars + 2 * kWMax, *aempty = afull + kAMaxStages;
   uint64_t *tfull = aempty + kAMaxStages, *tempty = tfull + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + 2);
+  uint64_t *drain = tempty + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   volatile uint32_t *err = tmem_slot + 1;
   // Which tile a weight stage belongs to (-1: no more tiles), and which tile each
   // accumulator holds, handed from the producer to the MMA issuer to the epilogue.
@@ -208,6 +220,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
       mb_init(&tfull[b], 2);  // the MMAs' completion and the issuer's tile hand-over
       mb_init(&tempty[b], kEpiThreads / 32);  // one arrival an epilogue warp
     }
+    mb_init(drain, 1);
     *err = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -354,11 +367,20 @@ __global__ void __launch_bounds__(kLmThreads, 1)
             sa = 0;
             if (!a_res) pa ^= 1u;
           }
+#ifdef TABBY_CHECKS
+          if (g == g_lm_checks.give_up) {
+            *err = 1u;
+            break;
+          }
+#endif
         }
         if (*err) break;
         mb_arrive(&tfull[b]);   // the tile number in acc_tile[b] is published
         mma_commit(&tfull[b]);  // the tile's accumulator is complete
       }
+      // Every product is done before the stages and TMEM go, also where a wait ran out.
+      mma_commit(drain);
+      mb_wait(drain, 0);
     }
   } else {
     // ---- epilogue: thread = token row (TMEM lane 32 * (warp % 4) + lane); the two warps
@@ -639,6 +661,9 @@ __global__ void __launch_bounds__(kLmThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (tid == 0) {
+#ifdef TABBY_CHECKS
+    if (!mb_test(drain, 0)) atomicAdd(&g_lm_checks.in_flight, 1);
+#endif
     if (*err) *a.error = a.epoch;
     // The last CTA to finish zeroes the tile counter for the next launch (every CTA has
     // taken its last tile by now).
@@ -895,5 +920,19 @@ int tabby_lmhead_sample_async(tabby_lmhead *h, const void *d_hidden, const void 
     return lfail(TABBY_ECUDA, "LM-head launch: %s", cudaGetErrorString(err));
   return TABBY_OK;
 }
+
+#ifdef TABBY_CHECKS
+// Sets the tile whose issuer gives up (-1: none) and gives the count of CTAs.
+TABBY_API int tabby_debug_lmhead(int32_t give_up, int32_t *in_flight) {
+  tabby::LmChecks c;
+  cudaError_t err = cudaMemcpyFromSymbol(&c, tabby::g_lm_checks, sizeof(c));
+  if (err == cudaSuccess) {
+    *in_flight = c.in_flight;
+    c = {give_up, 0};
+    err = cudaMemcpyToSymbol(tabby::g_lm_checks, &c, sizeof(c));
+  }
+  return (int)err;
+}
+#endif
 
 }  // extern "C"

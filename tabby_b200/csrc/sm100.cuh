@@ -46,6 +46,18 @@ __device__ __forceinline__ bool mb_try(uint64_t *b, uint32_t parity) {
       : "memory");
   return ok != 0u;
 }
+// Whether the phase of this parity is complete, without waiting.
+__device__ __forceinline__ bool mb_test(uint64_t *b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(b)), "r"(parity)
+      : "memory");
+  return ok != 0u;
+}
 // A bounded wait: false once it has run for kWaitNs.
 // The clock is read only once a first attempt has failed (reading it costs tens of ns).
 __device__ __forceinline__ bool mb_wait(uint64_t *b, uint32_t parity) {

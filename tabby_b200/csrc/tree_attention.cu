@@ -716,17 +716,7 @@ __global__ void __launch_bounds__(TreeCfg<DP, NS>::kThreads, NS == 1 ? 2 : 1)
   tc_fence_before();
   __syncthreads();
 #ifdef TABBY_CHECKS
-  if (tid == 0) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], 0;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_addr(drain))
-        : "memory");
-    if (!done) atomicAdd(&g_tree_checks.in_flight, 1);
-  }
+  if (tid == 0 && !mb_test(drain, 0)) atomicAdd(&g_tree_checks.in_flight, 1);
 #endif
   if (warp == 4 * NS + 1) {
     tc_fence_after();
