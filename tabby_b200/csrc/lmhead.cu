@@ -411,7 +411,8 @@ __global__ void __launch_bounds__(kLmThreads, 1)
       float thr_val = -INFINITY;  // bv[kFastKeep - 1]: a logit must exceed it to enter
       for (int t = 0;; t++) {
         const int b = t & 1;
-        if (!mb_wait(&tfull[b], (t >> 1) & 1)) {
+        // (The lanes of a warp learn the same outcome: the accumulator's loads need all of them.)
+        if (!__all_sync(0xffffffffu, mb_wait(&tfull[b], (t >> 1) & 1))) {
           *err = 1u;
           break;
         }
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
     };
     for (int t = 0;; t++) {
       const int b = t & 1;
-      if (!mb_wait(&tfull[b], (t >> 1) & 1)) {
+      if (!__all_sync(0xffffffffu, mb_wait(&tfull[b], (t >> 1) & 1))) {
         *err = 1u;
         break;
       }
