@@ -101,7 +101,8 @@ typedef struct tabby_state_layout {
  * in the first lengths[b] entries of every segment (all of them where d_lengths is NULL;
  * lengths are clipped to [0, entries]); later entries are left as they were. A row whose
  * parent is its own or lies outside [0, beams) is left as it was. h_states: n_states device
- * pointers, every state with the same layout, none overlapping another.
+ * pointers, every state with the same layout, none overlapping another. With n_states == 0 the
+ * other arguments are checked and nothing is done.
  * 1 <= beams <= TABBY_BEAM_MAX.
  */
 TABBY_API int tabby_states_reorder_async(int32_t device, void *const *h_states,

@@ -237,13 +237,22 @@ void reorder_states(const py::object &states, Tensor parents, std::optional<Tens
     need(*lengths, "lengths", at::kInt, {batch}, device);
     lengths = lengths->contiguous();
   }
-  for (const Group &g : groups_of(states, batch * beams, device, "states")) {
-    const tabby_state_layout l = layout_of(g.shape, g.stride, g.size, lengths.has_value());
+  const std::vector<Group> groups = groups_of(states, batch * beams, device, "states");
+  std::vector<tabby_state_layout> layouts;
+  auto call = [&](const tabby_state_layout &l, void *const *pointers, int32_t n) {
     check(tabby_states_reorder_async(
-        device.index(), g.pointers.data(), size32((int64_t)g.pointers.size(), "states"), &l,
-        size32(batch, "batch"), size32(beams, "beams"), parents.data_ptr<int32_t>(),
-        lengths ? lengths->data_ptr<int32_t>() : nullptr, stream_of(device)));
+        device.index(), pointers, n, &l, size32(batch, "batch"), size32(beams, "beams"),
+        parents.data_ptr<int32_t>(), lengths ? lengths->data_ptr<int32_t>() : nullptr,
+        stream_of(device)));
+  };
+  // All are checked before the first is moved: a call that raises has moved nothing.
+  for (const Group &g : groups) {
+    layouts.push_back(layout_of(g.shape, g.stride, g.size, lengths.has_value()));
+    size32((int64_t)g.pointers.size(), "states");
+    call(layouts.back(), nullptr, 0);
   }
+  for (size_t i = 0; i < groups.size(); i++)
+    call(layouts[i], groups[i].pointers.data(), (int32_t)groups[i].pointers.size());
 }
 
 // A tree's parents as [batch, nodes], a row of nodes for all.

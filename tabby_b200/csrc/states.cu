@@ -251,23 +251,25 @@ int tabby_states_reorder_async(int32_t device, void *const *h_states, int32_t n_
                        TABBY_BEAM_MAX, beams);
   const int st = check_layout("states_reorder", layout, (int64_t)batch * beams);
   if (st) return st;
+  ReorderArgs a;
+  a.l = merged(*layout);
+  // By the layout alone, whatever the pointers allow: a call without states tells whether one with
+  // states of this layout is refused. (Columns of a byte; wider ones are fewer.)
+  const double blocks = (double)batch * a.l.segments *
+                        std::ceil((double)a.l.entries * a.l.entry_bytes / kMoveThreads);
+  if (blocks > 2147483647.0)
+    return decode_fail(TABBY_EINVAL, "states_reorder: a state is too large for one launch");
   if (n_states == 0 || batch == 0) return TABBY_OK;
   if (!h_states || !d_parents)
     return decode_fail(TABBY_EINVAL, "states_reorder: states and parents must not be NULL");
   for (int32_t i = 0; i < n_states; i++)
     if (!h_states[i]) return decode_fail(TABBY_EINVAL, "states_reorder: state %d is NULL", i);
-  ReorderArgs a;
-  a.l = merged(*layout);
   const int w = vector_bytes(a.l, h_states, n_states, beams <= 16 ? 16 : beams <= 32 ? 8 : 4);
   a.beams = beams;
   a.parents = d_parents;
   a.lengths = d_lengths;
   a.vpe = (int32_t)(a.l.entry_bytes / w);
   a.packed = a.l.entries == 1 || a.l.entry_stride == a.l.entry_bytes;
-  const double blocks = (double)batch * a.l.segments *
-                        std::ceil((double)a.l.entries * a.vpe / kMoveThreads);
-  if (blocks > 2147483647.0)
-    return decode_fail(TABBY_EINVAL, "states_reorder: a state is too large for one launch");
   const int32_t most =
       (int32_t)std::min<double>(kMaxStates, std::max(1.0, 2147483647.0 / blocks));
   DeviceScope scope(device);

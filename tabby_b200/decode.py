@@ -96,6 +96,7 @@ def reorder_states(states: Union[torch.Tensor, Sequence[torch.Tensor]], parents:
     states: tensors [batch * beams, ...] of any type, or one tensor that stacks them along
     its first axis. With ``lengths`` ([batch] int32) they are caches [batch * beams, heads,
     entries, dim] (any strides, dim contiguous) and only the first lengths[b] entries move.
+    No state may overlap another. All are checked before the first is moved.
     """
     extension().reorder_states(states, parents, lengths)
 

@@ -127,6 +127,24 @@ def test_states_reorder_refuses():
     assert b"state 1 is NULL" in L.tabby_decode_last_error()
 
 
+def test_states_reorder_checks_without_states():
+    """What a call with states would refuse: the layout, and blocks past a launch's 2^31."""
+    m, L = _lib()
+
+    def call(lay, batch=2):
+        return L.tabby_states_reorder_async(0, None, 0, lay, batch, 2, P, None, None)
+
+    assert call(_layout(m)) == m.TABBY_OK
+    assert call(_layout(m, row=0)) == m.TABBY_EINVAL
+    assert b"overlap" in L.tabby_decode_last_error()
+    many = (1 << 31) - 1
+    assert call(_layout(m, row=many * 4, seg=4, ent=4, size=2, segments=many, entries=1)) \
+        == m.TABBY_EINVAL
+    assert b"too large" in L.tabby_decode_last_error()
+    assert call(_layout(m, row=many * 4, seg=4, ent=4, size=2, segments=many, entries=1), 1) \
+        == m.TABBY_OK
+
+
 def test_tree_accept_refuses():
     m, L = _lib()
     caches = (ctypes.c_void_p * 1)(None)

@@ -426,6 +426,23 @@ def test_reorder_refusals(tb):
     tb.reorder_states([x[:, :, :0]], p, lens)
 
 
+def test_reorder_that_is_refused_moves_nothing(tb):
+    """A state that cannot be moved, behind others that can: none of them is."""
+    p = random_parents(2, 3, 1)
+    lens = torch.tensor([5, 4], dtype=torch.int32, device="cuda")
+    x = filled((6, 2, 5, 8), torch.float32, 1)
+    y = filled((6, 3, 5, 16), torch.bfloat16, 2)
+    start = [x.clone(), y.clone()]
+    for bad, lengths in ((filled((6, 2, 9, 4), torch.float32, 3).transpose(2, 3), lens),
+                         (filled((1, 2, 5, 8), torch.int16, 3).expand(6, 2, 5, 8), lens),
+                         (filled((6, 7, 6, 5, 4), torch.int16, 3)[:, ::2, ::2, ::2], None),
+                         (filled((6, 2, 5), torch.int16, 3), lens)):
+        with pytest.raises((RuntimeError, ValueError)):
+            tb.reorder_states([x, y, bad], p, lengths)
+        for a, b in zip((x, y), start):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 # -- trees -----------------------------------------------------------------------------------
 def chain(parents, i):
     way = [i]
