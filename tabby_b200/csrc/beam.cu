@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   __shared__ uint32_t s_again[TABBY_BEAM_MAX], s_need;
   __shared__ double s_part[kMaxHelpers][TABBY_BEAM_MAX];
   __shared__ int s_count;
-  __shared__ uint32_t s_floor;
+  __shared__ uint32_t s_floor, s_top;
   const int b = blockIdx.x / a.helpers, helper = blockIdx.x - b * a.helpers;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row0 = b * a.beams, lists = a.beams * a.chunks;
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     if (tid > 0 && tid < a.helpers) store_cluster(in_cta(&s_need, tid), need);
     cluster_arrive();
   };
-  if (tid == 0) s_floor = 0;
+  if (tid == 0) s_floor = s_top = 0;
   // Log-sum-exps, a warp a beam.
   bool bad = false;
   for (int i = warp; i < a.beams; i += kWarps) {
@@ -543,15 +543,20 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     return c;
   };
   // A bound that at least n_out keys reach: the n_out-th largest of the threads' values (-inf
-  // where there are fewer), rounded down, by bisection over its upper 18 bits as fp32.
+  // where there are fewer), rounded down, by bisection over the exponent and 9 more bits, as fp32,
+  // of how far they lie below the prompt's best. (Of the keys themselves that many bits are steps
+  // of 4 to 16 where the running scores of long sequences lie, at minus some thousands: 32 x 8
+  // beams of 151936 at scores near -5000 take 42.6 us a step like this and 382 like that, 4 x 32
+  // of 49152, 64 out, 25.1 and 1113.)
   auto bound_of = [&](double top) {
-    const uint32_t key = order_key(__double2float_rd(top));
+    const double best = s_top > order_key(-INFINITY) ? (double)key_value(s_top) : 0.0;
+    const uint32_t key = order_key(__double2float_rd(__dsub_rd(top, best)));
     uint32_t kth = 0;
-    for (int bit = 31; bit >= 14; bit--) {
+    for (int bit = 30; bit >= 14; bit--) {  // the sign is known
       const uint32_t probe = kth | 1u << bit;
       if (__syncthreads_count(key >= probe) >= a.n_out) kth = probe;
     }
-    return kth > order_key(-INFINITY) ? (double)key_value(kth) : -INFINITY;
+    return kth > order_key(-INFINITY) ? __dadd_rd(best, (double)key_value(kth)) : -INFINITY;
   };
   auto keep = [&](const Cand &c, double least) {
     if (c.key < least) return;
@@ -633,8 +638,13 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     floor = fmax(floor, key_of(l, stats[l].floor));
   }
   const uint32_t floors = __reduce_max_sync(0xffffffffu, order_key(__double2float_rd(floor)));
-  if (lane == 0) atomicMax(&s_floor, floors);
-  double bound = bound_of(top);  // its barriers stand behind s_floor
+  const uint32_t tops = __reduce_max_sync(0xffffffffu, order_key(__double2float_ru(top)));
+  if (lane == 0) {
+    atomicMax(&s_floor, floors);
+    atomicMax(&s_top, tops);
+  }
+  __syncthreads();
+  double bound = bound_of(top);
   bound = fmax(bound, s_floor > order_key(-INFINITY) ? (double)key_value(s_floor) : -INFINITY);
   collect(bound);
   if (s_count > kPickTight) {
@@ -663,7 +673,8 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
   };
   const bool many = s_count > kPickCap;
   if (many) {
-    // Too many for the table, by ties: with all keys exact, the best one after the other.
+    // Too many for the table, by ties or near ties: with all keys exact, the best one after the
+    // other.
     __syncthreads();
     if (tid == 0) s_count = 0;
     for (int i = tid; i < a.beams; i += kThreads)

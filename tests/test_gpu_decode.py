@@ -205,6 +205,48 @@ def test_beam_step_large_values(tb):
     check_beam(tb.beam_step(x, scores, 6), plain_beam(x, scores, 6), 3001)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("batch,beams,vocab,n_out", [
+    (3, 8, 30000, 16), (2, 32, 20000, 64), (1, 4, 3001, 8), (2, 64, 2000, 128),
+])
+@pytest.mark.parametrize("offset", [-2.0 ** 12, -1e4, -3e7, 5e5])
+def test_beam_step_scores_of_long_sequences(tb, offset, batch, beams, vocab, n_out, dtype):
+    """Running scores far from 0, by thousands as after long sequences, and further."""
+    x, scores = beam_inputs(batch, beams, vocab, dtype, seed=vocab)
+    scores = scores + offset
+    check_beam(tb.beam_step(x, scores, n_out), plain_beam(x, scores, n_out), vocab)
+
+
+def graph_us(call, n=10):
+    """The median time of a call among others, in a graph."""
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(n):
+            call()
+    times = []
+    for _ in range(9):
+        a, z = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        graph.replay()
+        z.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(z) * 1e3 / n)
+    return sorted(times)[4]
+
+
+@pytest.mark.parametrize("batch,beams,vocab,n_out,dtype", [
+    (4, 32, 49152, 64, "f16"), (2, 32, 49152, 128, "f32"),
+])
+def test_beam_step_time_does_not_go_by_the_scores(tb, batch, beams, vocab, n_out, dtype):
+    """What a step has to look at may not grow with the scores' distance from 0 (where the bound
+    on the keys was coarse there, steps took 25 to 45 times as long)."""
+    x, scores = beam_inputs(batch, beams, vocab, dtype, seed=3)
+    near = graph_us(lambda: tb.beam_step(x, scores, n_out))
+    far = graph_us(lambda: tb.beam_step(x, scores - 8000, n_out))
+    assert far < 4 * near + 20, (near, far)
+
+
 def test_beam_step_strides_alignment_and_sharing(tb):
     g = gen(8)
     base = 4 * torch.randn(4 * 3 * 5000 + 64, device="cuda", generator=g)
