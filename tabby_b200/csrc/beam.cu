@@ -814,6 +814,23 @@ ScanPlan scan_plan(int64_t rows, int32_t vocab, int32_t dtype, int32_t n_out) {
   return p;
 }
 
+// Threads of a pick CTA. Many lists with many entries: more of them (rows of 50257 bf16, us a step
+// with 256 and with 1024 threads: 4 x 32 beams, 64 out 37.5 and 25.6; 32 x 8, 32 out 27.6 and 26.4;
+// 4 x 8, 16 out 13.1 and 14.6; 32 x 8, 16 out 23.2 and 24.0).
+int pick_threads(int32_t beams, int32_t n_out) { return beams * n_out >= 256 ? 1024 : 256; }
+// CTAs a prompt of the pick: where SMs are left over they help with the rare sums in 64 bits, as
+// many as find a place at once. A CTA of 1024 threads takes an SM, and a cluster of them has to lie
+// in one group of SMs: 15 clusters of 8 fit, 33 of 4. (4 beams, 64 out: 16 prompts with 8 CTAs each
+// 38.8 us a step, with 4 24.4; 64 prompts with 8, 4, 2 and 1 each 100, 53.1, 36.3 and 36.3; of a
+// step that needs the sums 145, 78.3, 56.2 and 69.3. CTAs of 256 threads, 64 x 4 beams, 8 out: 27.4
+// with 8 each, 21.4 with 4, 21.1 with 1, and 53.0, 48.4 and 84.6 with the sums.)
+int pick_helpers(int32_t batch, int threads) {
+  int n = kMaxHelpers;
+  // (The larger a cluster, the more SMs of the groups it leaves over.)
+  while (n > 1 && (int64_t)batch * n > (threads == 1024 ? 148 - 5 * n : 296)) n /= 2;
+  return n;
+}
+
 template <typename T>
 cudaError_t launch_beam(const BeamArgs &a, int nv, cudaStream_t q) {
   constexpr int kN = Vec16<T>::kN;
@@ -824,9 +841,7 @@ cudaError_t launch_beam(const BeamArgs &a, int nv, cudaStream_t q) {
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.batch * a.helpers));
-  // Many lists with many entries: more threads (4 x 32 beams, 64 out: 33.5 us a step with 256
-  // threads, 22.0 with 1024; 8 x 4, 64 out: 32.1 and 23.3; 32 x 8, 16 out: 34.2 and 52.0).
-  const int threads = a.beams * a.n_out >= 256 ? 1024 : 256;
+  const int threads = pick_threads(a.beams, a.n_out);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = q;
   cudaLaunchAttribute attr[2];
@@ -930,9 +945,7 @@ int tabby_beam_step_async(int32_t device, const void *d_logits, int32_t dtype,
   const ScanPlan plan = scan_plan((int64_t)rows, vocab, dtype, n_out);
   a.chunks = plan.chunks;
   a.cap = plan.cap;
-  // Where SMs are left over they help a prompt's CTA with the rare sums in 64 bits; otherwise they
-  // cost nothing (32 x 8 beams of 151936: 34.0 us a step without, 34.2 with).
-  a.helpers = batch <= 64 ? kMaxHelpers : batch <= 256 ? 2 : 1;
+  a.helpers = pick_helpers(batch, pick_threads(beams, n_out));
   a.gap = gap_of(vocab);
   a.stats = static_cast<ChunkStats *>(d_workspace);
   a.lists = reinterpret_cast<float2 *>(a.stats + rows * plan.chunks);

@@ -247,6 +247,19 @@ def test_beam_step_time_does_not_go_by_the_scores(tb, batch, beams, vocab, n_out
     assert far < 4 * near + 20, (near, far)
 
 
+@pytest.mark.parametrize("batch", [16, 32, 64])
+def test_beam_step_time_of_many_prompts(tb, batch):
+    """More of the pick's clusters than find a place at once run in waves of CTAs that only wait:
+    with 64 prompts steps took 2.8 times as long as with clusters that fit, with 16 1.6 times. A
+    batch's step stays below that of its halves, one after the other."""
+    x, scores = beam_inputs(batch, 4, 50257, "bf16", seed=3)
+    whole = graph_us(lambda: tb.beam_step(x, scores, 64))
+    h = batch // 2
+    half = graph_us(lambda: (tb.beam_step(x[:h], scores[:h], 64),
+                             tb.beam_step(x[h:], scores[h:], 64)))
+    assert whole < 0.8 * half, (whole, half)
+
+
 def test_beam_step_strides_alignment_and_sharing(tb):
     g = gen(8)
     base = 4 * torch.randn(4 * 3 * 5000 + 64, device="cuda", generator=g)
