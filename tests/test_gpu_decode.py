@@ -196,6 +196,28 @@ def test_beam_step_orders_keys_closer_than_fp32(tb):
     check_beam(tb.beam_step(x, scores, 8), want, vocab)
 
 
+@pytest.mark.parametrize("batch", [3, 30, 61, 100, 149, 257])
+@pytest.mark.parametrize("beams,vocab,n_out", [(31, 30000, 8), (4, 30000, 64)])
+def test_beam_step_clusters_of_every_size(tb, batch, beams, vocab, n_out):
+    """The second sums in 64 bits and the choice one by one, with 8, 4, 2 and 1 CTAs a prompt of
+    either size: prompts with keys closer than fp32 sums tell apart and prompts that are all tied,
+    among ordinary ones, so that clusters differ in whether they need help."""
+    x, scores = beam_inputs(3, beams, vocab, "f16", seed=beams)
+    x[0, 1] = x[0, 0]                       # keys about 1e-8 apart
+    low = int(x[0, 0].argmin())
+    x[0, 1, low] = x[0, 0, low] + 16
+    scores[0, :2] = -0.25
+    x[1] = 1.5                              # more ties than the table holds
+    scores[1] = -3.0
+    want = plain_beam(x, scores, n_out)
+    f = want["scores"][0]
+    assert (0 < -np.diff(f)).any() and (-np.diff(f)).min() < 1e-6
+    kind = np.random.RandomState(batch).randint(0, 3, batch)
+    kind[:3] = [2, 0, 1]
+    at = torch.from_numpy(kind).cuda()
+    check_beam(tb.beam_step(x[at], scores[at], n_out), {k: w[kind] for k, w in want.items()}, vocab)
+
+
 def test_beam_step_large_values(tb):
     x, scores = beam_inputs(3, 2, 3001, "f32", seed=2)
     x[0] *= 1e30
