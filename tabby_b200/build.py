@@ -6,7 +6,8 @@ libtabbysample.so (include/tabby_sample.h) is the sampler, libtabbydecode.so
 (include/tabby_decode.h) the decode operators for several hypotheses a sequence. Both are
 plain C-ABI shared objects that do not link against torch. CUDA's runtime is linked
 statically so they only need the driver. tabby_decode_torch.so is the Python side of the
-second on torch tensors (decode.py), an extension module built with g++ against torch.
+second on torch tensors (decode.py), an extension module built with g++ against torch; where
+either is missing it is left out with a note, since the libraries need neither.
 """
 from __future__ import annotations
 
@@ -82,19 +83,31 @@ def _build_lib(lib_path: str, sources: list, verbose: bool, defines: tuple) -> N
 def _build_torch() -> None:
     import sysconfig
 
-    import torch
-    from torch.utils import cpp_extension
-
+    gxx = shutil.which("g++")
+    missing = "" if gxx else "g++"
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:
+        missing = "torch"
+    else:
+        if torch.version.cuda is None:
+            missing = "torch with CUDA"
+    if missing:
+        sys.stderr.write(f"{missing} is missing: {os.path.basename(DECODE_TORCH)} is not built "
+                         "(tabby_b200.decode needs it)\n")
+        return
     libs = cpp_extension.library_paths()
-    includes = [os.path.join(ROOT, "include"), "/usr/local/cuda/include",
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    includes = [os.path.join(ROOT, "include"), os.path.join(cuda, "include"),
                 sysconfig.get_paths()["include"], *cpp_extension.include_paths()]
     tmp = DECODE_TORCH + ".tmp"
-    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    _run([gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
           "-DTORCH_EXTENSION_NAME=tabby_decode_torch",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
           *[f"-I{i}" for i in includes], os.path.join(CSRC, "decode_torch.cpp"), "-o", tmp,
-          f"-L{LIBDIR}", "-l:libtabbydecode.so", *[f"-L{p}" for p in libs], "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
-          "-lc10", "-lc10_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"],
+          f"-L{LIBDIR}", "-l:libtabbydecode.so", *[f"-L{p}" for p in libs], "-ltorch",
+          "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"],
          "g++ failed for decode_torch.cpp")
     os.replace(tmp, DECODE_TORCH)
 
