@@ -177,8 +177,9 @@ struct Group {
 };
 
 // Groups of states with one layout each: of one tensor that stacks them or a sequence of them.
+// Those without an element are left out and counted.
 std::vector<Group> groups_of(const py::object &states, int64_t rows, at::Device device,
-                             const std::string &name) {
+                             const std::string &name, int64_t *empty = nullptr) {
   std::vector<Group> groups;
   auto check_rows = [&](const Tensor &x, int64_t axis) {
     if (x.device() != device)
@@ -190,7 +191,10 @@ std::vector<Group> groups_of(const py::object &states, int64_t rows, at::Device 
   if (THPVariable_Check(states.ptr())) {
     const Tensor &x = THPVariable_Unpack(states.ptr());
     check_rows(x, 1);
-    if (x.numel() == 0) return groups;
+    if (x.numel() == 0) {
+      if (empty) *empty = x.size(0);
+      return groups;
+    }
     if (x.size(0) > 1 && x.stride(0) == 0) value_error(name + " overlap");
     Group g;
     g.shape.assign(x.sizes().begin() + 1, x.sizes().end());
@@ -205,7 +209,10 @@ std::vector<Group> groups_of(const py::object &states, int64_t rows, at::Device 
     if (!THPVariable_Check(h.ptr())) type_error(name + " must be tensors");
     const Tensor &x = THPVariable_Unpack(h.ptr());
     check_rows(x, 0);
-    if (x.numel() == 0) continue;
+    if (x.numel() == 0) {
+      if (empty) ++*empty;
+      continue;
+    }
     Group *at = nullptr;
     for (Group &g : groups)
       if (g.size == (int64_t)x.element_size() && at::IntArrayRef(g.shape) == x.sizes() &&
@@ -337,12 +344,12 @@ py::tuple tree_accept(const Tensor &sampled, Tensor tokens, Tensor parents, Tens
   need(lengths, "lengths", at::kInt, {batch}, device);
   tokens = tokens.contiguous();
   lengths = lengths.contiguous();
-  const std::vector<Group> groups = groups_of(caches, batch, device, "caches");
+  int64_t empty = 0;
+  const std::vector<Group> groups = groups_of(caches, batch, device, "caches", &empty);
   if (groups.size() > 1) value_error("the caches must share one layout");
   tabby_state_layout l = {};
   // (Without a cache no slot lies past the end: one without an entry is not the same.)
-  if (groups.empty() && batch > 0 && py::len(caches) > 0)
-    value_error("the caches must not be empty");
+  if (empty > 0 && batch > 0) value_error("the caches must not be empty");
   if (!groups.empty()) l = layout_of(groups[0].shape, groups[0].stride, groups[0].size, true);
   const Tensor all = fresh({batch * (nodes + 3)}, at::kInt, device);
   Tensor path = part(all, 0, {batch, nodes}, at::kInt);

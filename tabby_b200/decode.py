@@ -127,7 +127,7 @@ def tree_accept(sampled: torch.Tensor, tokens: torch.Tensor, parents: torch.Tens
     sampled [batch, nodes] int32 in any strides: the token chosen after each slot; tokens
     [batch, nodes] int32: the drafted ones; parents [batch, nodes] or [nodes] as in
     tree_attention; caches: [batch, heads, entries, dim] each, or one tensor that stacks
-    them. ``lengths`` itself is not changed: the new ones are returned.
+    them, all of one shape, type and strides. ``lengths`` itself is not changed: the new ones are returned.
     """
     return TreeAccept(*extension().tree_accept(sampled, tokens, parents, lengths, caches))
 

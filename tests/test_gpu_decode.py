@@ -937,6 +937,17 @@ def test_tree_accept_refusals(tb):
         tb.tree_accept(w, w, w, lens)
 
 
+def test_tree_accept_refuses_an_empty_cache_among_others(tb):
+    z = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    c = filled((2, 2, 9, 8), torch.float32, 1)
+    for caches in ([c, c[:, :, :0]], [c[:, :, :0], c], c[None, :, :, :0]):
+        with pytest.raises(ValueError):
+            tb.tree_accept(z, z, z, lens, caches)
+    none = tb.tree_accept(z, z, z - 1, lens, c[None][:0])  # of no layers: no cache
+    assert none.counts.tolist() == [1, 1]
+
+
 # -- together --------------------------------------------------------------------------------
 def test_beam_search_with_a_cache(tb):
     """Eight steps of a beam search over a toy model whose logits depend on the whole cached
