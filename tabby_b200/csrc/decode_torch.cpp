@@ -11,6 +11,7 @@
 #include <cmath>
 #include <optional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "tabby_decode.h"
@@ -169,6 +170,21 @@ tabby_state_layout layout_of(at::IntArrayRef shape, at::IntArrayRef stride, int6
   return l;
 }
 
+// Whether elements of a tensor share memory: taken from the smallest stride up, each must pass
+// what the ones below it span. (The library's check of a layout, with the axis of a stack.)
+bool overlaps(const Tensor &x) {
+  std::vector<std::pair<int64_t, int64_t>> axes;  // stride, size
+  for (int64_t i = 0; i < x.dim(); i++)
+    if (x.size(i) > 1) axes.push_back({x.stride(i), x.size(i)});
+  std::sort(axes.begin(), axes.end());
+  int64_t span = 1;
+  for (const auto &a : axes) {
+    if (a.first < span) return true;
+    span += a.first * (a.second - 1);
+  }
+  return false;
+}
+
 // States of one shape, type and strides.
 struct Group {
   at::DimVector shape, stride;
@@ -195,7 +211,7 @@ std::vector<Group> groups_of(const py::object &states, int64_t rows, at::Device 
       if (empty) *empty = x.size(0);
       return groups;
     }
-    if (x.size(0) > 1 && x.stride(0) == 0) value_error(name + " overlap");
+    if (overlaps(x)) value_error(name + " overlap");
     Group g;
     g.shape.assign(x.sizes().begin() + 1, x.sizes().end());
     g.stride.assign(x.strides().begin() + 1, x.strides().end());

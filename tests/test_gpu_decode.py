@@ -503,6 +503,25 @@ def test_reorder_refusals(tb):
     tb.reorder_states([x[:, :, :0]], p, lens)
 
 
+def test_stacks_that_overlap_are_refused(tb):
+    p = random_parents(2, 3, 1)
+    lens = torch.tensor([5, 4], dtype=torch.int32, device="cuda")
+    z = torch.zeros(6, 4, dtype=torch.int32, device="cuda")
+    x = filled((9, 2, 5, 8), torch.float32, 1)
+    start = x.clone()
+    for bad in (x[:6].expand(3, 6, 2, 5, 8), x.unfold(0, 6, 1).permute(0, 4, 1, 2, 3),
+                x.unfold(2, 4, 1)[:6].permute(3, 0, 1, 2, 4)):
+        with pytest.raises(ValueError):
+            tb.reorder_states(bad, p, lens)
+        with pytest.raises(ValueError):
+            tb.tree_accept(z, z, z - 1, torch.zeros(6, dtype=torch.int32, device="cuda"), bad)
+    assert torch.equal(x.view(torch.int32), start.view(torch.int32))
+    stack = filled((6, 2, 3, 5, 8), torch.float32, 2).transpose(1, 2).permute(2, 0, 1, 3, 4)
+    want = torch.stack([plain_reorder(s, p, lens) for s in stack])
+    tb.reorder_states(stack, p, lens)  # two states between whose heads the other's lie
+    assert torch.equal(stack.contiguous().view(torch.int32), want.view(torch.int32))
+
+
 def test_reorder_that_is_refused_moves_nothing(tb):
     """A state that cannot be moved, behind others that can: none of them is."""
     p = random_parents(2, 3, 1)
