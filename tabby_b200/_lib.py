@@ -196,9 +196,3 @@ def decode_lib() -> ctypes.CDLL:
 def check(status: int) -> None:
     if status != TABBY_OK:
         raise TabbyError(status, lib().tabby_last_error().decode(errors="replace"))
-
-
-def check_decode(status: int) -> None:
-    if status != TABBY_OK:
-        raise TabbyError(status,
-                         decode_lib().tabby_decode_last_error().decode(errors="replace"))

@@ -681,7 +681,6 @@ __global__ void __launch_bounds__(kLmThreads, 1)
   }
 }
 
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link to libcuda).
 // K-major bf16 matrix [outer][inner] with boxes of 64 x box_rows (inner x outer), 128-byte
 // swizzle, zero fill out of bounds.
 bool make_map(CUtensorMap *m, const void *ptr, uint64_t inner, uint64_t outer, uint32_t box_rows) {

@@ -199,6 +199,7 @@ using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t,
                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no link to libcuda).
 EncodeTiled encode_fn() {
   static std::once_flag once;
   static EncodeTiled fn = nullptr;
