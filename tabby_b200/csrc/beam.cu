@@ -40,8 +40,8 @@ struct ChunkStats {
   float floor; // n_out logits of the chunk are no smaller (-inf: there may be fewer)
   int32_t count;
 };
-// More keys than this are worth a tighter bound (12 x 5 beams, first steps among them: 16.0 us a
-// step with 256, 15.8 with 128, 16.9 with 64; 4 x 32 beams: 22.0, 22.0 and 30.7).
+// More keys than this are worth a tighter bound (12 x 5 beams, first steps among them: 15.5 us a
+// step with 256, 15.4 with 128, 16.5 with 64; 4 x 32 beams: 23.9, 23.7 and 31.9; over 16 inputs).
 constexpr int kPickTight = 128;
 
 struct BeamArgs {
@@ -543,16 +543,16 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const __grid_consta
     return c;
   };
   // A bound that at least n_out keys reach: the n_out-th largest of the threads' values (-inf
-  // where there are fewer), rounded down, by bisection over the exponent and 9 more bits, as fp32,
-  // of how far they lie below the prompt's best. (Of the keys themselves that many bits are steps
-  // of 4 to 16 where the running scores of long sequences lie, at minus some thousands: 32 x 8
-  // beams of 151936 at scores near -5000 take 42.6 us a step like this and 382 like that, 4 x 32
-  // of 49152, 64 out, 25.1 and 1113.)
+  // where there are fewer), rounded down, by bisection over the exponent and 8 more bits, as fp32,
+  // of how far they lie below the prompt's best. (Of the keys themselves as many bits are steps
+  // of 8 to 32 where the running scores of long sequences lie, at minus some thousands: at scores
+  // near -5000 32 x 8 beams of 151936 take 42.6 us a step like this and took 382 by the keys, one
+  // bit more of them even; 4 x 32 of 49152, 64 out, 25.1 and 1113.)
   auto bound_of = [&](double top) {
     const double best = s_top > order_key(-INFINITY) ? (double)key_value(s_top) : 0.0;
     const uint32_t key = order_key(__double2float_rd(__dsub_rd(top, best)));
     uint32_t kth = 0;
-    for (int bit = 30; bit >= 14; bit--) {  // the sign is known
+    for (int bit = 30; bit >= 15; bit--) {  // the sign is known
       const uint32_t probe = kth | 1u << bit;
       if (__syncthreads_count(key >= probe) >= a.n_out) kth = probe;
     }
