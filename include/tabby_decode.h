@@ -60,8 +60,10 @@ TABBY_API const char *tabby_decode_last_error(void);
  * d_logits: dtype, element (b, i, v) at b * batch_stride + i * beam_stride + v (elements; the
  * strides may be 0 to share rows), aligned to its type. d_finished may be NULL (none is; then
  * eos_id may be -1: no end token); d_next_finished may be NULL.
- * Scores are exact to (3 ln(vocab) + 24) 2^-24 and their rounding to f32; parents and tokens are
- * those of 64-bit keys.
+ * Scores are exact to (3 ln(vocab) + 24) 2^-24 and their rounding to f32. Parents and tokens are
+ * those of keys with log-sum-exps good to 3e-13 and the rounding of 64-bit sums: continuations of
+ * different beams whose keys lie closer together than about 1e-12 may change places, unless the
+ * beams' logits and scores are alike (then they tie).
  * 1 <= beams <= TABBY_BEAM_MAX, 1 <= n_out <= TABBY_BEAM_MAX_OUT, 1 <= vocab <= 2^30,
  * beams * vocab < 2^31; batch * beams * vocab below 2^42 or so (a launch's 2^31 blocks).
  * d_workspace: tabby_beam_workspace_bytes bytes, 16-byte aligned.
@@ -125,7 +127,10 @@ TABBY_API int tabby_states_reorder_async(int32_t device, void *const *h_states,
  * then, at entries lengths[b] + j, the keys and values of its tree's slots (written before the
  * call). Slot j in use attends to the whole context, to itself and to its ancestors:
  *   out[b][j][h] = sum_t p_t v[b][h'][t],  p = softmax over those t of scale * q[b][j][h].k[b][h'][t]
- * with h' = h / (heads / kv_heads); statistics and sums in fp32, out rounded once to the type.
+ * with h' = h / (heads / kv_heads). Scores, statistics and sums are in fp32; the weights (before
+ * their division by the sum) are rounded to the type where they meet v, which takes 16-bit
+ * operands, and out is rounded to it once. Both together put out off by about 2.2e-3 (bf16) or
+ * 2.9e-4 (fp16) relative in the norm, where the rounding of out alone is 1.7e-3 and 2.1e-4.
  * Slots not in use give 0. One slot (nodes == 1) is the ordinary decode step. Keys and values
  * of the context and of the slots in use must be finite; what the cache holds elsewhere does
  * not matter. Element (b, h, t) of k starts at b * k_batch_stride + h * k_head_stride +
@@ -134,7 +139,8 @@ TABBY_API int tabby_states_reorder_async(int32_t device, void *const *h_states,
  * kv_heads; pointers 16-byte aligned and strides multiples of 8 elements.
  * A cache's axis longer than one has a stride of its own (no shared sequences or heads).
  * parents_stride is the number of ints between the sequences' trees (0: one tree for all).
- * Should a device-side wait run out of its bound (0.5 s), the outputs it concerns are NaN.
+ * Should a device-side wait run out of its bound (0.5 s), the outputs it concerns are NaN, and so
+ * are those that the same block of threads had still to compute.
  */
 #define TABBY_TREE_MAX_DIM 128
 typedef struct tabby_tree_attention_args {
@@ -174,7 +180,7 @@ TABBY_API int tabby_tree_attention_async(int32_t device, const tabby_tree_attent
  *   next_lengths  lengths + counts
  * and in every cache entry lengths[b] + r takes what entry lengths[b] + path[r] held, r <
  * counts, in place; all other entries are left as they were. The caches' rows are the
- * sequences; n_caches may be 0 (then layout is NULL and no slot lies past the end).
+ * sequences; all have the one layout; n_caches may be 0 (then layout is NULL and no slot lies past the end).
  */
 TABBY_API int tabby_tree_accept_async(int32_t device, const int32_t *d_sampled,
                                       int64_t sampled_batch_stride, int64_t sampled_stride,

@@ -3,7 +3,8 @@
 The calls of include/tabby_decode.h on torch tensors. All of them are asynchronous on the
 current stream of the tensors' device, take and give device tensors, allocate through
 PyTorch (so they can be captured in a CUDA graph) and keep nothing between calls. They take no
-part in autograd.
+part in autograd; the calls that work in place do not count the tensors' versions up, so autograd
+does not notice that a tensor it has saved was moved.
 
 Beam search, one step:
 
@@ -75,7 +76,8 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, n_out: Optional[int] =
     logits [batch, beams, vocab] float32, bfloat16 or float16 (rows may be strided or shared),
     scores [batch, beams] float32. -inf logits are banned tokens, -inf scores dead beams; a
     ``finished`` beam [batch, beams] goes on with ``eos_id`` at its score. Missing
-    continuations have parent and token -1 and score -inf. A prompt whose live beams hold NaN
+    continuations have parent and token -1 and score -inf. Keys of different beams closer than
+    about 1e-12 may change places unless the beams are alike. A prompt whose live beams hold NaN
     or +inf has status TABBY_EINPUT and no continuations.
     """
     return BeamStep(*extension().beam_step(logits, scores, n_out, finished, eos_id))
@@ -113,7 +115,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     entries, dim] in any strides with dim contiguous (16-byte aligned rows); lengths [batch]
     int32; parents [batch, nodes] or [nodes] int32, -1 for a root, lower for unused slots.
     nodes <= 64, dim a multiple of 8 up to 128, heads a multiple of kv_heads. scale defaults
-    to dim ** -0.5. One slot (parents -1) is the ordinary decode step.
+    to dim ** -0.5. One slot (parents -1) is the ordinary decode step. The softmax is in float32;
+    its weights are rounded to the caches' type where they meet the values, the output once.
     """
     return extension().tree_attention(q, k_cache, v_cache, lengths, parents, scale)
 
