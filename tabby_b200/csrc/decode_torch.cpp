@@ -64,12 +64,11 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
   return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
 
-// A tensor in the storage of `whole`, from element `first` (of its own type) on: outputs share an
-// allocation, without a view's bookkeeping.
-Tensor part(const Tensor &whole, int64_t first, at::IntArrayRef sizes, at::ScalarType type) {
+// A tensor in the storage of `whole`, from element `first` on: outputs of one type share an
+// allocation, without a view's bookkeeping. (Of several types they could not be saved together.)
+Tensor part(const Tensor &whole, int64_t first, at::IntArrayRef sizes) {
   Tensor t = at::detail::make_tensor<c10::TensorImpl>(
-      c10::TensorImpl::VIEW, c10::Storage(whole.storage()), whole.key_set(),
-      c10::scalarTypeToTypeMeta(type));
+      c10::TensorImpl::VIEW, c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
   t.unsafeGetTensorImpl()->set_storage_offset(first);
   t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
   return t;
@@ -113,12 +112,12 @@ py::tuple beam_step(Tensor logits, Tensor scores, std::optional<int64_t> n_out_o
   check(tabby_beam_workspace_bytes(size32(batch, "batch"), size32(beams, "beams"),
                                    size32(vocab, "vocab"), size32(n_out, "n_out"), &bytes));
   const int64_t n = batch * n_out;
-  const Tensor all = fresh({13 * n + 4 * batch}, at::kByte, device);
-  Tensor next_scores = part(all, 0, {batch, n_out}, at::kFloat);
-  Tensor parents = part(all, n, {batch, n_out}, at::kInt);
-  Tensor tokens = part(all, 2 * n, {batch, n_out}, at::kInt);
-  Tensor status = part(all, 3 * n, {batch}, at::kInt);
-  Tensor ends = part(all, 12 * n + 4 * batch, {batch, n_out}, at::kBool);
+  Tensor next_scores = fresh({batch, n_out}, at::kFloat, device);
+  const Tensor all = fresh({2 * n + batch}, at::kInt, device);
+  Tensor parents = part(all, 0, {batch, n_out});
+  Tensor tokens = part(all, n, {batch, n_out});
+  Tensor status = part(all, 2 * n, {batch});
+  Tensor ends = fresh({batch, n_out}, at::kBool, device);
   Tensor work = fresh({(int64_t)bytes}, at::kByte, device);
   check(tabby_beam_step_async(
       device.index(), logits.data_ptr(), dtype, logits.stride(0), logits.stride(1),
@@ -368,10 +367,10 @@ py::tuple tree_accept(const Tensor &sampled, Tensor tokens, Tensor parents, Tens
   if (empty > 0 && batch > 0) value_error("the caches must not be empty");
   if (!groups.empty()) l = layout_of(groups[0].shape, groups[0].stride, groups[0].size, true);
   const Tensor all = fresh({batch * (nodes + 3)}, at::kInt, device);
-  Tensor path = part(all, 0, {batch, nodes}, at::kInt);
-  Tensor counts = part(all, batch * nodes, {batch}, at::kInt);
-  Tensor next_tokens = part(all, batch * (nodes + 1), {batch}, at::kInt);
-  Tensor next_lengths = part(all, batch * (nodes + 2), {batch}, at::kInt);
+  Tensor path = part(all, 0, {batch, nodes});
+  Tensor counts = part(all, batch * nodes, {batch});
+  Tensor next_tokens = part(all, batch * (nodes + 1), {batch});
+  Tensor next_lengths = part(all, batch * (nodes + 2), {batch});
   check(tabby_tree_accept_async(
       device.index(), sampled.data_ptr<int32_t>(), sampled.stride(0), sampled.stride(1),
       tokens.data_ptr<int32_t>(), parents.data_ptr<int32_t>(), outer(parents, 0),

@@ -14,6 +14,8 @@ Tolerances. u = 2^-24.
   running sums in fp32 add (n / 8 + 16) 2^-23 A over n keys; ex2 of an argument up to S adds
   (4 + 3 * 2 S) u, twice.
 """
+import copy
+import io
 import math
 import os
 import subprocess
@@ -965,6 +967,27 @@ def test_tree_accept_refuses_an_empty_cache_among_others(tb):
             tb.tree_accept(z, z, z, lens, caches)
     none = tb.tree_accept(z, z, z - 1, lens, c[None][:0])  # of no layers: no cache
     assert none.counts.tolist() == [1, 1]
+
+
+def test_outputs_are_ordinary_tensors(tb):
+    """Saved and loaded together, copied, changed in place and used in autograd."""
+    x, scores = beam_inputs(2, 3, 50, "f32")
+    z = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
+    for r in (tb.beam_step(x.requires_grad_(), scores), tb.tree_accept(z, z, z - 1, z[:, 0])):
+        f = io.BytesIO()
+        torch.save(list(r), f)
+        f.seek(0)
+        for a, b, c in zip(r, torch.load(f), copy.deepcopy(list(r))):
+            assert a.dtype == b.dtype and torch.equal(a, b) and torch.equal(a, c)
+            assert not a.requires_grad
+        others = [t.clone() for t in r[1:]]
+        r[0].fill_(1)
+        assert all(torch.equal(a, b) for a, b in zip(others, r[1:]))
+    step = tb.beam_step(x, scores)
+    (step.scores.requires_grad_() * 2).sum().backward()
+    assert (step.scores.grad == 2).all()
+    with torch.inference_mode():
+        tb.beam_step(x, scores).scores.add_(1)
 
 
 # -- together --------------------------------------------------------------------------------
